@@ -7,4 +7,4 @@ Python mirror of that interface plus the GGUF reader / synthetic-model writer.
 from . import _lib, gguf  # noqa: F401
 from ._lib import SpecDecError, lib  # noqa: F401
 
-__all__ = ["gguf", "dequant", "engine", "lib", "SpecDecError"]
+__all__ = ["gguf", "dequant", "engine", "paged", "lib", "SpecDecError"]

@@ -49,6 +49,26 @@ class GenParams(C.Structure):
                 ("reuse_draft_kv", C.c_int)]
 
 
+class Pages(C.Structure):
+    _fields_ = [("table", C.c_void_p), ("held", C.c_void_p), ("free_pages", C.c_void_p), ("n_free", C.c_void_p),
+                ("n_req", C.c_int), ("table_ld", C.c_int), ("n_pages", C.c_int), ("page_size", C.c_int)]
+
+
+class KvPool(C.Structure):
+    _fields_ = [("k", C.c_void_p), ("v", C.c_void_p), ("page_stride", C.c_int64), ("pos_stride", C.c_int64),
+                ("head_stride", C.c_int64), ("n_pages", C.c_int), ("page_size", C.c_int), ("n_kv_heads", C.c_int),
+                ("head_dim", C.c_int), ("dtype", C.c_int)]
+
+
+class AttnArgs(C.Structure):
+    _fields_ = [("pool", KvPool), ("q", C.c_void_p), ("out", C.c_void_p), ("q_ld", C.c_int64), ("q_head", C.c_int64),
+                ("out_ld", C.c_int64), ("out_head", C.c_int64), ("table", C.c_void_p), ("kv_len", C.c_void_p),
+                ("q_start", C.c_void_p), ("q_len", C.c_void_p), ("prefix_table", C.c_void_p), ("alibi", C.c_void_p),
+                ("n_tokens", C.c_int), ("n_heads", C.c_int), ("n_req", C.c_int), ("table_ld", C.c_int),
+                ("max_q", C.c_int), ("max_kv", C.c_int), ("prefix_len", C.c_int), ("window", C.c_int),
+                ("scale", C.c_float), ("softcap", C.c_float), ("workspace", C.c_void_p), ("workspace_bytes", C.c_size_t)]
+
+
 class GenStats(C.Structure):
     _fields_ = [("n_generated", C.c_int), ("total_draft", C.c_int64), ("total_accepted", C.c_int64),
                 ("total_iterations", C.c_int64), ("ms_prefill", C.c_double), ("ms_decode", C.c_double)]
@@ -62,7 +82,7 @@ class BatchStats(C.Structure):
 
 BATCH_MAX_WIDTH = 8
 
-vp, i32, f32, sz, u64 = C.c_void_p, C.c_int, C.c_float, C.c_size_t, C.c_uint64
+vp, i32, f32, sz, u64, i64 = C.c_void_p, C.c_int, C.c_float, C.c_size_t, C.c_uint64, C.c_int64
 _SIGS = {
     "sd_last_error": (C.c_char_p, []),
     "sd_abi_version": (i32, []),
@@ -81,6 +101,11 @@ _SIGS = {
     "sd_host_q4_0_q8_0_matvec": (None, [vp, vp, vp, i32, i32]),
     "sd_host_kq_matvec": (None, [i32, vp, vp, vp, i32, i32]),
     "sd_host_cache_clear": (None, []),
+    "sd_pages_reset_dev": (i32, [vp, vp]),
+    "sd_pages_plan_dev": (i32, [vp, vp, vp, i32, i32, i32, vp, vp, vp, vp, vp]),
+    "sd_kv_append_dev": (i32, [vp, vp, vp, i32, i64, i64, vp, i32, vp]),
+    "sd_attention_workspace": (sz, [vp]),
+    "sd_attention_dev": (i32, [vp, vp]),
     "sd_ctx_opts_default": (None, [vp]),
     "sd_nccl_unique_id": (i32, [vp]),
     "sd_nccl_comm_create": (i32, [vp, i32, i32, i32, vp]),

@@ -1,0 +1,336 @@
+// sd_paged.cu -- pages of a K/V cache shared by many requests: block tables and slot maps from request lengths,
+// and K/V rows written through the slot map.
+#include <cooperative_groups.h>
+#include <cuda_bf16.h>
+
+#include <algorithm>
+
+#include "sd_common.cuh"
+#include "sd_host.h"
+#include "sd_paged.h"
+
+namespace cg = cooperative_groups;
+using namespace sd;
+
+namespace sd {
+
+int check_pages(const sd_pages* p, const char* what) {
+    if (!p || !p->table || !p->held || !p->free_pages || !p->n_free) return fail(SD_ERR_INVALID, "%s: null argument", what);
+    if (p->n_req < 1 || p->n_req > SD_PAGES_MAX_REQ)
+        return fail(SD_ERR_INVALID, "%s: n_req %d outside 1..%d", what, p->n_req, SD_PAGES_MAX_REQ);
+    if (p->page_size < SD_PAGE_MIN || p->page_size > SD_PAGE_MAX || (p->page_size & (p->page_size - 1)))
+        return fail(SD_ERR_INVALID, "%s: page_size %d is not a power of two in %d..%d", what, p->page_size, SD_PAGE_MIN, SD_PAGE_MAX);
+    if (p->table_ld < 1 || (int64_t)p->table_ld * p->page_size > INT32_MAX || (int64_t)p->table_ld * p->n_req > INT32_MAX)
+        return fail(SD_ERR_INVALID, "%s: table_ld %d", what, p->table_ld);
+    if (p->n_pages < 1 || (int64_t)p->n_pages * p->page_size > INT32_MAX)
+        return fail(SD_ERR_INVALID, "%s: n_pages %d", what, p->n_pages);
+    return SD_OK;
+}
+
+int check_kv_pool(const sd_kv_pool* p, const char* what) {
+    if (!p || !p->k || !p->v) return fail(SD_ERR_INVALID, "%s: null pool", what);
+    if (p->page_size < SD_PAGE_MIN || p->page_size > SD_PAGE_MAX || (p->page_size & (p->page_size - 1)))
+        return fail(SD_ERR_INVALID, "%s: page_size %d is not a power of two in %d..%d", what, p->page_size, SD_PAGE_MIN, SD_PAGE_MAX);
+    if (p->n_pages < 1 || (int64_t)p->n_pages * p->page_size > INT32_MAX)
+        return fail(SD_ERR_INVALID, "%s: n_pages %d", what, p->n_pages);
+    if (p->n_kv_heads < 1 || p->n_kv_heads > 1024 || p->head_dim < 8 || p->head_dim > 256 || p->head_dim % 8)
+        return fail(SD_ERR_INVALID, "%s: %d heads of %d", what, p->n_kv_heads, p->head_dim);
+    if (p->dtype != SD_F16 && p->dtype != SD_BF16) return fail(SD_ERR_INVALID, "%s: pool dtype %d", what, p->dtype);
+    if (p->page_stride < 1 || p->pos_stride < 1 || p->head_stride < p->head_dim)
+        return fail(SD_ERR_INVALID, "%s: pool strides", what);
+    return SD_OK;
+}
+
+int paged_device(const void* p, const char* what, int* dev) {
+    int cur = -1;
+    cudaError_t e = cudaGetDevice(&cur);
+    if (e != cudaSuccess) {
+        cudaGetLastError();
+        return fail(SD_ERR_NO_DEVICE, "%s: %s", what, cudaGetErrorString(e));
+    }
+    cudaPointerAttributes at{};
+    if ((e = cudaPointerGetAttributes(&at, p)) != cudaSuccess) return cuda_fail(e, what);
+    if (at.type != cudaMemoryTypeDevice && at.type != cudaMemoryTypeManaged)
+        return fail(SD_ERR_INVALID, "%s: not device memory", what);
+    if (at.type == cudaMemoryTypeDevice && at.device != cur)
+        return fail(SD_ERR_INVALID, "%s: the current device is %d but the arrays live on device %d", what, cur, at.device);
+    *dev = cur;
+    return SD_OK;
+}
+
+namespace {
+
+// ---------------------------------------------------------------------------------------------
+// Page plan.  All of a step is three prefix sums over the requests (surplus pages, wanted pages, new tokens) and
+// three scatters.  Latency bound: a step moves a few bytes per request and token, so everything is one launch of one
+// cluster.  Every CTA of the cluster computes the sums for itself (cheaper than handing them over), then the
+// scatters are dealt over the cluster's threads, each finding its request by bisection in shared memory.  Cluster
+// barriers separate reading the old state, pushing, taking and reading the new table; a step that moves no page
+// passes none.
+// ---------------------------------------------------------------------------------------------
+constexpr int kPlanThreads = 512;
+
+struct PlanArgs {
+    int32_t *table, *held, *free_pages, *n_free;
+    int n_req, table_ld, n_pages, page_size;
+    const int32_t *kv_len, *q_len;
+    int q_stride, pos0, n_tokens;
+    int32_t *q_start, *slots, *positions, *missing;
+    int* err;
+};
+
+// Last b in [0, n) with start[b] <= k (start ascends, start[0] = 0).
+__device__ __forceinline__ int owner(const int* start, int n, int k) {
+    int lo = 0, hi = n;
+    while (hi - lo > 1) {
+        const int m = (lo + hi) >> 1;
+        if (start[m] <= k) lo = m; else hi = m;
+    }
+    return lo;
+}
+
+__global__ void __launch_bounds__(kPlanThreads) k_pages_plan(const PlanArgs a) {
+    extern __shared__ int sm[];
+    __shared__ int wsum[3][kPlanThreads / 32];
+    const int n = a.n_req, tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    int* back = sm;               // [n + 1] exclusive sums of surplus pages
+    int* want = back + n + 1;     // of wanted pages
+    int* toks = want + n + 1;     // of new tokens
+    int* base = toks + n + 1;     // [n] first page that is given back or taken: min(held, needed)
+    const cg::cluster_group cluster = cg::this_cluster();
+    const int gtid = (int)cluster.block_rank() * kPlanThreads + tid, gn = (int)cluster.num_blocks() * kPlanThreads;
+    const int cap = a.table_ld * a.page_size;
+    const int count0 = *a.n_free;
+
+    // sums: each thread takes `per` consecutive requests
+    const int per = (n + kPlanThreads - 1) / kPlanThreads;
+    const int b0 = min(n, tid * per), b1 = min(n, b0 + per);
+    int s[3] = {0, 0, 0};
+    bool bad = false;
+    for (int b = b0; b < b1; ++b) {
+        int kv = a.kv_len[b], q = a.q_len[b];
+        if (kv < 0 || kv > cap) bad = true, kv = min(max(kv, 0), cap);
+        const int q_max = a.q_stride > 0 ? a.q_stride : a.n_tokens;
+        if (q < 0 || q > q_max) bad = true, q = min(max(q, 0), q_max);
+        if (a.q_stride > 0 && q > 0 && b * a.q_stride + q > a.n_tokens) bad = true;
+        const int need = (kv + a.page_size - 1) / a.page_size, had = min(max(a.held[b], 0), a.table_ld);
+        const int v[3] = {max(had - need, 0), max(need - had, 0), q};
+        back[b] = v[0], want[b] = v[1], toks[b] = v[2];
+        base[b] = min(had, need);
+#pragma unroll
+        for (int i = 0; i < 3; ++i) s[i] += v[i];
+    }
+    int incl[3];
+#pragma unroll
+    for (int i = 0; i < 3; ++i) {
+        incl[i] = s[i];
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+            const int u = __shfl_up_sync(0xffffffffu, incl[i], o);
+            if (lane >= o) incl[i] += u;
+        }
+        if (lane == 31) wsum[i][warp] = incl[i];
+    }
+    __syncthreads();
+    int tot[3];
+#pragma unroll
+    for (int i = 0; i < 3; ++i) {
+        int before = 0, all = 0;
+#pragma unroll
+        for (int w = 0; w < kPlanThreads / 32; ++w) {
+            const int u = wsum[i][w];
+            before += w < warp ? u : 0;
+            all += u;
+        }
+        tot[i] = all;
+        int run = before + incl[i] - s[i];
+        int* arr = i == 0 ? back : i == 1 ? want : toks;
+        for (int b = b0; b < b1; ++b) {
+            const int v = arr[b];
+            arr[b] = run;
+            run += v;
+        }
+        if (tid == 0) arr[n] = all;
+    }
+    __syncthreads();
+    const int n_back = tot[0], n_want = tot[1], n_tok = tot[2];
+    const int count = min(count0 + n_back, a.n_pages), left = max(count - n_want, 0);
+    if (n_back | n_want) {
+        cluster.sync();  // every CTA has read the old state
+        for (int k = gtid; k < n_back; k += gn) {
+            const int b = owner(back, n, k);
+            const size_t i = (size_t)b * a.table_ld + base[b] + (k - back[b]);
+            if (count0 + k < a.n_pages) a.free_pages[count0 + k] = a.table[i];
+            a.table[i] = -1;
+        }
+        if (n_back && n_want) cluster.sync();  // what was given back can be taken
+        for (int k = gtid; k < n_want; k += gn) {
+            if (k >= count) break;
+            const int b = owner(want, n, k);
+            a.table[(size_t)b * a.table_ld + base[b] + (k - want[b])] = a.free_pages[count - 1 - k];
+            a.free_pages[count - 1 - k] = -1;
+        }
+        for (int b = gtid; b < n; b += gn) {
+            const int w = want[b + 1] - want[b];
+            a.held[b] = base[b] + min(max(count - want[b], 0), w);
+        }
+        if (gtid == 0) *a.n_free = left;
+        cluster.sync();  // the new table
+    }
+    if (gtid == 0) {
+        if (a.missing) *a.missing = max(n_want - count, 0);
+        if (a.q_stride == 0 && n_tok > a.n_tokens) bad = true;
+    }
+    for (int b = gtid; b < n; b += gn) a.q_start[b] = a.q_stride > 0 ? b * a.q_stride : toks[b];
+    for (int k = gtid; k < a.n_tokens; k += gn) {
+        int b, t;
+        bool live;
+        if (a.q_stride > 0) {
+            b = k / a.q_stride;
+            t = k - b * a.q_stride;
+            live = b < n;
+        } else {
+            b = owner(toks, n, k);
+            t = k - toks[b];
+            live = true;
+        }
+        int slot = -1, pos = -1;
+        if (live && t >= 0 && t < toks[b + 1] - toks[b]) {
+            const int p = min(a.kv_len[b], cap) - (toks[b + 1] - toks[b]) + t;
+            if (p >= 0 && p < cap) {
+                pos = a.pos0 + p;
+                const int page = a.table[(size_t)b * a.table_ld + p / a.page_size];
+                if (page >= 0) slot = page * a.page_size + p % a.page_size;
+            }
+        }
+        a.slots[k] = slot;
+        if (a.positions) a.positions[k] = pos;
+    }
+    if (bad) set_dev_error(a.err, DEV_ERR_BAD_ARG);
+}
+
+__global__ void k_pages_reset(sd_pages p) {
+    const size_t n_tab = (size_t)p.n_req * p.table_ld, step = (size_t)gridDim.x * blockDim.x;
+    for (size_t i = (size_t)blockIdx.x * blockDim.x + threadIdx.x; i < n_tab; i += step) p.table[i] = -1;
+    for (size_t i = (size_t)blockIdx.x * blockDim.x + threadIdx.x; i < (size_t)p.n_pages; i += step)
+        p.free_pages[i] = p.n_pages - 1 - (int)i;
+    for (size_t i = (size_t)blockIdx.x * blockDim.x + threadIdx.x; i < (size_t)p.n_req; i += step) p.held[i] = 0;
+    if (blockIdx.x == 0 && threadIdx.x == 0) *p.n_free = p.n_pages;
+}
+
+// ---------------------------------------------------------------------------------------------
+// K/V append: a cast copy, bound by HBM (source read once, pool rows written once).
+// ---------------------------------------------------------------------------------------------
+struct AppendArgs {
+    const void *k, *v;
+    void *kp, *vp;
+    int64_t k_ld, v_ld, page_stride, pos_stride, head_stride;
+    int n_kv, hd, page_size, n_slots, n_tokens;
+    const int32_t* slots;
+    int* err;
+};
+
+__device__ __forceinline__ float to_f32(float x) { return x; }
+__device__ __forceinline__ float to_f32(__half x) { return __half2float(x); }
+__device__ __forceinline__ float to_f32(__nv_bfloat16 x) { return __bfloat162float(x); }
+template <class T> __device__ __forceinline__ T from_f32(float x);
+template <> __device__ __forceinline__ __half from_f32<__half>(float x) { return __float2half_rn(x); }
+template <> __device__ __forceinline__ __nv_bfloat16 from_f32<__nv_bfloat16>(float x) { return __float2bfloat16_rn(x); }
+
+template <class S, class T>
+__global__ void __launch_bounds__(256) k_kv_append(const AppendArgs a) {
+    const int row = a.n_kv * a.hd;
+    const long long total = (long long)a.n_tokens * row, step = (long long)gridDim.x * blockDim.x;
+    for (long long i = (long long)blockIdx.x * blockDim.x + threadIdx.x; i < total; i += step) {
+        const int tok = (int)(i / row), e = (int)(i - (long long)tok * row);
+        const int slot = a.slots[tok];
+        if (slot < 0 || slot >= a.n_slots) {
+            if (slot != -1 && e == 0) set_dev_error(a.err, DEV_ERR_BAD_ARG);
+            continue;
+        }
+        const int h = e / a.hd, d = e - h * a.hd;
+        const size_t dst = (size_t)(slot / a.page_size) * a.page_stride + (size_t)(slot % a.page_size) * a.pos_stride +
+                           (size_t)h * a.head_stride + d;
+        static_cast<T*>(a.kp)[dst] = from_f32<T>(to_f32(static_cast<const S*>(a.k)[(size_t)tok * a.k_ld + e]));
+        static_cast<T*>(a.vp)[dst] = from_f32<T>(to_f32(static_cast<const S*>(a.v)[(size_t)tok * a.v_ld + e]));
+    }
+}
+
+}  // namespace
+}  // namespace sd
+
+extern "C" {
+
+int sd_pages_reset_dev(const sd_pages* p, void* stream) {
+    clear_error();
+    int rc = check_pages(p, "sd_pages_reset_dev"), dev;
+    if (rc || (rc = paged_device(p->table, "sd_pages_reset_dev", &dev))) return rc;
+    k_pages_reset<<<device_sm_count(dev), 256, 0, (cudaStream_t)stream>>>(*p);
+    const cudaError_t e = cudaGetLastError();
+    return e == cudaSuccess ? SD_OK : cuda_fail(e, "pages reset");
+}
+
+int sd_pages_plan_dev(const sd_pages* p, const int32_t* kv_len, const int32_t* q_len, int q_stride, int pos0, int n_tokens,
+                      int32_t* q_start, int32_t* slots, int32_t* positions, int32_t* missing, void* stream) {
+    clear_error();
+    int rc = check_pages(p, "sd_pages_plan_dev"), dev;
+    if (rc) return rc;
+    if (!kv_len || !q_len || !q_start || n_tokens < 0 || (n_tokens > 0 && !slots) || q_stride < 0 || pos0 < 0)
+        return fail(SD_ERR_INVALID, "sd_pages_plan_dev: bad arguments");
+    if ((int64_t)p->n_req * q_stride > INT32_MAX || (int64_t)pos0 + (int64_t)p->table_ld * p->page_size > INT32_MAX)
+        return fail(SD_ERR_INVALID, "sd_pages_plan_dev: q_stride %d or pos0 %d too large", q_stride, pos0);
+    if ((rc = paged_device(p->table, "sd_pages_plan_dev", &dev))) return rc;
+    PlanArgs a{p->table, p->held, p->free_pages, p->n_free, p->n_req, p->table_ld, p->n_pages, p->page_size,
+               kv_len, q_len, q_stride, pos0, n_tokens, q_start, slots, positions, missing, device_error_word(dev)};
+    const size_t smem = ((size_t)4 * p->n_req + 3) * sizeof(int);
+    cudaError_t e = cudaSuccess;
+    if (smem > 48 * 1024 - 1024)
+        e = cudaFuncSetAttribute(k_pages_plan, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+    if (e != cudaSuccess) return cuda_fail(e, "pages plan");
+    const int items = std::max(n_tokens, p->n_req);
+    int ctas = 1;
+    while (ctas < 8 && ctas * kPlanThreads < items) ctas *= 2;
+    cudaLaunchConfig_t cfg{};
+    cfg.gridDim = dim3(ctas);
+    cfg.blockDim = dim3(kPlanThreads);
+    cfg.dynamicSmemBytes = smem;
+    cfg.stream = (cudaStream_t)stream;
+    cudaLaunchAttribute at{};
+    at.id = cudaLaunchAttributeClusterDimension;
+    at.val.clusterDim.x = ctas;
+    at.val.clusterDim.y = at.val.clusterDim.z = 1;
+    cfg.attrs = &at;
+    cfg.numAttrs = 1;
+    e = cudaLaunchKernelEx(&cfg, k_pages_plan, (const PlanArgs)a);
+    return e == cudaSuccess ? SD_OK : cuda_fail(e, "pages plan");
+}
+
+int sd_kv_append_dev(const sd_kv_pool* pool, const void* k, const void* v, int src_dtype, int64_t k_ld, int64_t v_ld,
+                     const int32_t* slots, int n_tokens, void* stream) {
+    clear_error();
+    int rc = check_kv_pool(pool, "sd_kv_append_dev"), dev;
+    if (rc) return rc;
+    if (!k || !v || !slots || n_tokens < 0) return fail(SD_ERR_INVALID, "sd_kv_append_dev: bad arguments");
+    if (src_dtype != SD_F32 && src_dtype != pool->dtype)
+        return fail(SD_ERR_INVALID, "sd_kv_append_dev: source type %d for a pool of type %d", src_dtype, pool->dtype);
+    if (n_tokens == 0) return SD_OK;
+    if ((rc = paged_device(pool->k, "sd_kv_append_dev", &dev))) return rc;
+    const int row = pool->n_kv_heads * pool->head_dim;
+    AppendArgs a{k, v, pool->k, pool->v, k_ld, v_ld, pool->page_stride, pool->pos_stride, pool->head_stride,
+                 pool->n_kv_heads, pool->head_dim, pool->page_size, pool->n_pages * pool->page_size, n_tokens, slots,
+                 device_error_word(dev)};
+    const long long total = (long long)n_tokens * row;
+    const int grid = (int)std::min<long long>((total + 255) / 256, 16LL * device_sm_count(dev));
+    const cudaStream_t st = (cudaStream_t)stream;
+    if (pool->dtype == SD_F16) {
+        if (src_dtype == SD_F32) k_kv_append<float, __half><<<grid, 256, 0, st>>>(a);
+        else k_kv_append<__half, __half><<<grid, 256, 0, st>>>(a);
+    } else {
+        if (src_dtype == SD_F32) k_kv_append<float, __nv_bfloat16><<<grid, 256, 0, st>>>(a);
+        else k_kv_append<__nv_bfloat16, __nv_bfloat16><<<grid, 256, 0, st>>>(a);
+    }
+    const cudaError_t e = cudaGetLastError();
+    return e == cudaSuccess ? SD_OK : cuda_fail(e, "kv append");
+}
+
+}  // extern "C"

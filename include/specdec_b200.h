@@ -128,6 +128,96 @@ SD_API void sd_host_kq_matvec(int type, const void *W, const float *x, float *y,
 SD_API void sd_host_cache_clear(void);
 
 /* ======================================================================================
+ * Paged K/V cache: pages shared by many requests, and attention over them.  No reference counterpart (the
+ * reference keeps one ring per process, mistral/kv_cache.h:10-57); sd_batch_create_shared below serves streams
+ * that share a prompt prefix through it.
+ *
+ * All arrays are device memory of the current device, all calls are stream-ordered, allocate nothing and can be
+ * captured into a CUDA graph.  What only the device knows (lengths, page ids, slots) is checked there: an entry out
+ * of range is left out as each call says and records DEV error 3, which sd_device_error reads.
+ * ====================================================================================== */
+enum { SD_F32 = 0, SD_F16 = 1, SD_BF16 = 2 };
+#define SD_PAGES_MAX_REQ 8192
+#define SD_PAGE_MIN 16
+#define SD_PAGE_MAX 256
+
+/* Who holds which page.  Request b holds held[b] pages, table[b * table_ld .. + held[b]) in order, -1 behind them;
+ * free_pages[0 .. *n_free) is the stack of free pages, -1 above it.  page_size: a power of two in 16..256;
+ * n_pages * page_size < 2^31; n_req <= SD_PAGES_MAX_REQ. */
+typedef struct {
+    int32_t *table;      /* [n_req][table_ld] */
+    int32_t *held;       /* [n_req] */
+    int32_t *free_pages; /* [n_pages] */
+    int32_t *n_free;     /* [1] */
+    int n_req, table_ld, n_pages, page_size;
+} sd_pages;
+
+/* Every page free (the next one taken is page 0), no request holds any. */
+SD_API int sd_pages_reset_dev(const sd_pages *p, void *stream);
+
+/* One step's block tables and slot map from request lengths.  kv_len [n_req]: positions of each request after this
+ * step; q_len [n_req]: how many of them, at the end, are new in it.
+ * Pages: requests that need fewer than they hold push the surplus on the free stack, in ascending (request, page)
+ * order; then those that need more take pages from its top, in the same order.  Where the stack runs out the entry
+ * stays -1 and *missing (if not NULL) counts it; the request holds what it got and asks again in the next step.
+ * Tokens: the new positions of request b are tokens q_start[b] .. q_start[b] + q_len[b) of the step, packed one
+ * request after another (q_stride 0) or at b * q_stride (q_len <= q_stride).  slots [n_tokens]: token's slot in the
+ * pool, page * page_size + offset; positions [n_tokens] (or NULL): pos0 + its position.  Tokens of no request get -1
+ * in both; a position that has no page gets slot -1, one before 0 (q_len > kv_len) -1 in both.
+ * q_len = 0 keeps a request's pages, kv_len = 0 releases them.  A length past table_ld * page_size is cut there, a
+ * q_len outside 0 .. q_stride to that range, tokens past n_tokens are dropped; each records DEV error 3. */
+SD_API int sd_pages_plan_dev(const sd_pages *p, const int32_t *kv_len, const int32_t *q_len, int q_stride, int pos0,
+                             int n_tokens, int32_t *q_start, int32_t *slots, int32_t *positions, int32_t *missing,
+                             void *stream);
+
+/* K and V of n_pages pages of page_size positions; strides in elements, the same for both:
+ * element (page, pos, head, d) at page * page_stride + pos * pos_stride + head * head_stride + d. */
+typedef struct {
+    void *k, *v;
+    int64_t page_stride, pos_stride, head_stride;
+    int n_pages, page_size, n_kv_heads, head_dim;
+    int dtype; /* SD_F16 or SD_BF16 */
+} sd_kv_pool;
+
+/* Write token i's K and V rows ([n_kv_heads][head_dim], heads head_dim apart, tokens k_ld / v_ld elements apart) into
+ * slot slots[i], rounded to the pool's type.  src_dtype: SD_F32 or the pool's.  Slot -1 is skipped, any other slot
+ * outside the pool is skipped and recorded.  Slots of one call must differ: of tokens with the same slot an
+ * unspecified mix stays. */
+SD_API int sd_kv_append_dev(const sd_kv_pool *pool, const void *k, const void *v, int src_dtype, int64_t k_ld,
+                            int64_t v_ld, const int32_t *slots, int n_tokens, void *stream);
+
+/* Attention of the new tokens of n_req requests over the pages: grouped heads, every request's own positions behind
+ * one prefix that all of them share (stored once, read once for all rows).
+ * Row t of request b (token q_start[b] + t, t < q_len[b]) is at own position i = kv_len[b] - q_len[b] + t and sees the
+ * prefix_len positions of prefix_table and the own positions 0 .. i of table[b * table_ld ..], whose distance from it
+ * is below `window` (0: no limit).  Its scores are scale * q.k, then softcap * tanh(score / softcap) if softcap > 0,
+ * then - alibi[head] * distance if alibi is not NULL; softmax and the weighted sum of V are accumulated in fp32, the
+ * softmax weights enter the product with V in the pool's type.
+ * A row with i < 0, or with nothing to see, is 0.  Tokens of no request are left as they were.  Positions whose page
+ * id is outside the pool are not seen (recorded, unless all that every row of the call would see of the page is
+ * outside the window).  K and V of positions that no row sees may hold anything; those that some row of the request
+ * sees must be finite.
+ * q_start ascends, the ranges do not overlap and end within n_tokens.  max_q and max_kv bound q_len and kv_len on the
+ * host (they size the launch; a tight max_kv gives the better split); a longer request is cut there (recorded).
+ * head_dim a multiple of 8 up to 256, n_heads a multiple of n_kv_heads, q and out of the pool's type. */
+typedef struct {
+    sd_kv_pool pool;
+    const void *q;
+    void *out;
+    int64_t q_ld, q_head, out_ld, out_head; /* elements between tokens, between heads */
+    const int32_t *table, *kv_len, *q_start, *q_len;
+    const int32_t *prefix_table; /* [ceil(prefix_len / page_size)], NULL if prefix_len is 0 */
+    const float *alibi;          /* [n_heads] or NULL */
+    int n_tokens, n_heads, n_req, table_ld, max_q, max_kv, prefix_len, window;
+    float scale, softcap;
+    void *workspace; /* sd_attention_workspace(a) bytes, 256-byte aligned; one call at a time uses it */
+    size_t workspace_bytes;
+} sd_attn_args;
+/* Workspace bytes of a call with these sizes (its pointers are not read); 0 may be passed as NULL. */
+SD_API size_t sd_attention_workspace(const sd_attn_args *a);
+SD_API int sd_attention_dev(const sd_attn_args *a, void *stream);
+
+/* ======================================================================================
  * Model context: weights in HBM, fp16 KV ring, verify / decode forward, generation loops
  * ====================================================================================== */
 
