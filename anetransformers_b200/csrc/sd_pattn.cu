@@ -5,9 +5,11 @@
 //   z_j = f(scale q_t.k_j) - slope (pos_t - pos_j),  f(s) = cap tanh(s / cap) or s
 // over the visible j: prefix positions, then the request's own positions up to the row's, less those at a distance
 // of `window` or more.
+#include <cuda.h>
 #include <cuda_bf16.h>
 
 #include <algorithm>
+#include <type_traits>
 
 #include "sd_common.cuh"
 #include "sd_host.h"
@@ -98,6 +100,944 @@ __global__ void __launch_bounds__(128) k_pattn_general(const sd_attn_args a, int
         if (lane + 32 * i < hd) out[lane + 32 * i] = pa_from<T>(acc[i] * inv);
 }
 
+
+// ---------------------------------------------------------------------------------------------
+// Tensor-core kernel (head_dim 64 and 128): tcgen05.mma with S, P and O in tensor memory, K/V tiles by TMA.
+//
+// Rows.  The query rows of one kv head are (token, head of its group); a tile holds TPT = 128 / G tokens, TPT * G
+// rows of the MMA's M = 128.  Keys come in tiles of 128.  Work items:
+//   own items      (request, row tiles, kv head, chunk of its keys)
+//   prefix items   (row tiles over the whole step's tokens, kv head, chunk of the prefix): the shared prefix is read
+//                  once for the rows of all requests.  A request with more rows than two tiles fills them by itself
+//                  and takes the prefix tiles in front of its own ("inline", one softmax over both).
+// An item of more than TPT tokens is a pair: slot 0 and 1 (accumulators and softmax warpgroups) take a row tile
+// each and share every K/V tile.  A smaller one has one row tile: slot 0 takes its even key tiles, slot 1 the odd
+// ones, and slot 0 merges the two states at the end.  Rows whose keys lie in several items leave (max, sum, O) in
+// the workspace for k_pattn_combine; others are written by their item.
+//
+// Warps (12): 0-3 softmax of slot 0, 4-7 of slot 1 (thread = row), 8 TMA, 9 MMA issue, 10 zeroes V rows that no row
+// may see (0 x NaN is NaN in the product), 11 idle.  P overwrites S in tensor memory and is the A operand of P V.
+// The running maximum that O refers to moves only when a row's maximum rises by more than 2^8 (exact: O and the sum
+// refer to the same value), so O is rarely rescaled.  Every wait is bounded in time (sd_common.cuh).
+// ---------------------------------------------------------------------------------------------
+constexpr int kPaThreads = 384;
+constexpr int kPaKeys = 128;        // keys per tile
+constexpr int kPaHalf = 128 * 128;  // bytes of 128 rows x 64 elements (one 128-byte swizzle row each)
+
+struct PaArgs {
+    CUtensorMap tq, tk, tv;
+    sd_attn_args a;
+    int G, TPT;            // query heads per kv head, tokens per row tile
+    int np;                // key tiles of the prefix
+    int n_pt, cp, ct_pre;  // prefix items: row-tile pairs over the tokens, chunks, tiles per chunk
+    int ct_own;            // tiles per chunk of own items
+    float* acc;            // [splits][n_tokens * n_heads][hd]
+    float2* ml;            // [splits][n_tokens * n_heads]
+    int* err;
+};
+
+struct PaCtl {
+    uint64_t qfull, qempty;
+    uint64_t full[8], empty[8], fixed[8];
+    uint64_t sfull[2], pready[2], ofull[2];
+    uint64_t mready, mdone, done;
+    uint32_t okmask[16];  // per key tile, in turn: which of its 16-key groups were loaded
+    float2 ml1[128];      // slot 1's state at a merge
+    uint32_t tmem;
+    int abort;
+    int wsum[16];
+};
+
+struct PaItem {
+    int b, kvh, tok0, ntok;   // request (-1: prefix item), kv head, first token, tokens
+    bool pair, direct;
+    int v0, n, npt;           // first key tile, their number; tiles below npt are the prefix's
+    int klo_p, klo_o, khi_o;  // keys outside [klo_p, prefix_len) and [klo_o, khi_o) are seen by no row of the item
+    int base;                 // kv - q: own position of the request's first row
+    int q0, rows;             // the request's first token and its tokens
+    int split;
+};
+
+__device__ __forceinline__ int pa_q(const sd_attn_args& a, int b) { return min(max(a.q_len[b], 0), a.max_q); }
+__device__ __forceinline__ int pa_kv(const sd_attn_args& a, int b) { return min(max(a.kv_len[b], 0), a.max_kv); }
+__device__ __forceinline__ int pa_rows(const sd_attn_args& a, int b) {
+    return max(0, min(pa_q(a, b), a.n_tokens - max(a.q_start[b], 0)));
+}
+__device__ __forceinline__ bool pa_inline(const PaArgs& p, int rows) { return p.a.prefix_len > 0 && rows > 2 * p.TPT; }
+__device__ __forceinline__ int pa_tiles(const PaArgs& p, int rows) {
+    return rows <= p.TPT ? (rows > 0) : (rows + 2 * p.TPT - 1) / (2 * p.TPT);
+}
+__device__ __forceinline__ int pa_chunks(const PaArgs& p, int kv, bool inl) {
+    const int t = (kv + kPaKeys - 1) / kPaKeys + (inl ? p.np : 0);
+    return max(1, (t + p.ct_own - 1) / p.ct_own);
+}
+__device__ __forceinline__ int pa_request(const sd_attn_args& a, int tok) {
+    int lo = 0, hi = a.n_req;
+    while (hi - lo > 1) {
+        const int m = (lo + hi) >> 1;
+        if (a.q_start[m] <= tok) lo = m; else hi = m;
+    }
+    return lo;
+}
+
+// Item number i of the launch; false if it holds nothing (prefix rows of an inline request).
+__device__ __forceinline__ bool pa_item(const PaArgs& p, const int* ustart, int i, PaItem& it) {
+    const sd_attn_args& a = p.a;
+    const int n_kv = a.pool.n_kv_heads, P = a.prefix_len, W = a.window;
+    const int n_pre = p.cp * p.n_pt * n_kv;
+    if (i < n_pre) {
+        it.kvh = i % n_kv;
+        const int u = i / n_kv, c = u / p.n_pt;
+        it.tok0 = (u - c * p.n_pt) * 2 * p.TPT;
+        it.ntok = min(2 * p.TPT, a.n_tokens - it.tok0);
+        if (a.max_q > 2 * p.TPT) {
+            const int b = pa_request(a, it.tok0), rows = pa_rows(a, b);
+            if (pa_inline(p, rows) && it.tok0 >= a.q_start[b] && it.tok0 + it.ntok <= a.q_start[b] + rows) return false;
+        }
+        it.b = -1;
+        it.pair = it.ntok > p.TPT;
+        it.direct = false;
+        it.npt = p.np;
+        it.klo_p = W > 0 ? max(0, P + 1 - W) : 0;
+        it.klo_o = it.khi_o = 0;
+        it.v0 = max(c * p.ct_pre, it.klo_p / kPaKeys);
+        it.n = max(0, min(p.np, (c + 1) * p.ct_pre) - it.v0);
+        if (it.klo_p >= P) it.n = 0;
+        it.base = it.q0 = it.rows = 0;
+        it.split = c;
+        return true;
+    }
+    i -= n_pre;
+    it.kvh = i % n_kv;
+    const int u = i / n_kv;
+    int lo = 0, hi = a.n_req;
+    while (hi - lo > 1) {
+        const int m = (lo + hi) >> 1;
+        if (ustart[m] <= u) lo = m; else hi = m;
+    }
+    const int b = lo, local = u - ustart[b];
+    const int q = pa_q(a, b), kv = pa_kv(a, b), rows = pa_rows(a, b), nt = pa_tiles(p, rows);
+    const bool inl = pa_inline(p, rows);
+    const int c = local / nt, tile = nt - 1 - (local - c * nt);  // the tiles with most keys first
+    const int chunks = pa_chunks(p, kv, inl);
+    it.b = b;
+    it.q0 = max(a.q_start[b], 0);
+    it.rows = rows;
+    it.base = kv - q;
+    it.tok0 = it.q0 + tile * 2 * p.TPT;
+    it.ntok = min(2 * p.TPT, rows - tile * 2 * p.TPT);
+    it.pair = it.ntok > p.TPT;
+    it.direct = chunks == 1 && (P == 0 || inl);
+    it.npt = inl ? p.np : 0;
+    const int first = it.base + tile * 2 * p.TPT, last = first + it.ntok - 1;
+    it.khi_o = max(0, last + 1);
+    it.klo_o = W > 0 ? max(0, first + 1 - W) : 0;
+    it.klo_p = W > 0 ? min(P, max(0, P + first + 1 - W)) : 0;
+    int s0 = it.klo_o / kPaKeys + it.npt;
+    if (inl && it.klo_p < P) s0 = it.klo_p / kPaKeys;
+    it.v0 = max(c * p.ct_own, s0);
+    const int end = min((c + 1) * p.ct_own, it.npt + (it.khi_o + kPaKeys - 1) / kPaKeys);
+    it.n = last < 0 ? 0 : max(0, end - it.v0);
+    it.split = p.cp + c;
+    return true;
+}
+
+// Keys [k0, k0 + 128) of virtual tile v of the item, and which of them its rows may see.
+struct PaTile {
+    bool prefix;
+    int k0, lo, hi;
+};
+__device__ __forceinline__ PaTile pa_tile(const PaArgs& p, const PaItem& it, int v) {
+    PaTile t;
+    t.prefix = v < it.npt;
+    t.k0 = (t.prefix ? v : v - it.npt) * kPaKeys;
+    t.lo = t.prefix ? it.klo_p : it.klo_o;
+    t.hi = t.prefix ? p.a.prefix_len : it.khi_o;
+    return t;
+}
+
+__device__ __forceinline__ bool pa_wait(uint64_t* bar, uint32_t parity, PaCtl* ctl, int* err, int code) {
+    if (*(volatile int*)&ctl->abort) return false;
+    if (mbar_wait(bar, parity)) return true;
+    set_dev_error(err, code);
+    *(volatile int*)&ctl->abort = 1;
+    return false;
+}
+__device__ __forceinline__ bool pa_wait_warp(uint64_t* bar, uint32_t parity, PaCtl* ctl, int* err, int code) {
+    return __all_sync(0xffffffffu, pa_wait(bar, parity, ctl, err, code));
+}
+
+__device__ __forceinline__ void tma_3d(uint32_t dst, const CUtensorMap* m, int x, int y, int z, uint64_t* bar) {
+    asm volatile(
+        "cp.async.bulk.tensor.3d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5}], [%2];" ::"r"(dst),
+        "l"(m), "r"(smem_u32(bar)), "r"(x), "r"(y), "r"(z)
+        : "memory");
+}
+__device__ __forceinline__ void tma_4d(uint32_t dst, const CUtensorMap* m, int x, int y, int z, int w, uint64_t* bar) {
+    asm volatile(
+        "cp.async.bulk.tensor.4d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5, %6}], [%2];" ::"r"(dst),
+        "l"(m), "r"(smem_u32(bar)), "r"(x), "r"(y), "r"(z), "r"(w)
+        : "memory");
+}
+
+// Shared-memory matrix descriptor of a 128-byte swizzled operand (rows of 64 16-bit elements): start address, leading
+// and stride byte offsets in 16-byte units, bit 46 the descriptor version of sm_100, bits 61-63 the swizzle.
+// K-major (Q, K): stride = 1024 between groups of 8 rows.  MN-major (V, read by columns): leading = the distance
+// between blocks of 64 columns, stride = 1024 between groups of 8 keys.
+__device__ __forceinline__ uint64_t sw128_desc(uint32_t addr, uint32_t lbo, uint32_t sbo) {
+    return (uint64_t)((addr >> 4) & 0x3FFFu) | ((uint64_t)((lbo >> 4) & 0x3FFFu) << 16) |
+           ((uint64_t)((sbo >> 4) & 0x3FFFu) << 32) | (1ull << 46) | (2ull << 61);
+}
+// Instruction descriptor of kind::f16: D fp32, A and B fp16 or bf16, B MN-major if trans_b, M = 128.
+__host__ __device__ constexpr uint32_t idesc_f16(bool bf16, int n, bool trans_b) {
+    return (1u << 4) | ((bf16 ? 1u : 0u) << 7) | ((bf16 ? 1u : 0u) << 10) | ((trans_b ? 1u : 0u) << 16) |
+           ((uint32_t)(n >> 3) << 17) | ((uint32_t)(128 >> 4) << 24);
+}
+__device__ __forceinline__ void mma_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t acc) {
+    asm volatile(
+        "{\n .reg .pred p;\n setp.ne.b32 p, %4, 0;\n"
+        " tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n}\n" ::"r"(d),
+        "l"(a), "l"(b), "r"(idesc), "r"(acc)
+        : "memory");
+}
+__device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, uint32_t acc) {
+    asm volatile(
+        "{\n .reg .pred p;\n setp.ne.b32 p, %4, 0;\n"
+        " tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n}\n" ::"r"(d),
+        "r"(a), "l"(b), "r"(idesc), "r"(acc)
+        : "memory");
+}
+__device__ __forceinline__ void pa_commit(uint64_t* bar) {
+    asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(smem_u32(bar))
+                 : "memory");
+}
+__device__ __forceinline__ void pa_fence_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
+__device__ __forceinline__ void pa_fence_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
+__device__ __forceinline__ void pa_ld32(uint32_t taddr, uint32_t (&v)[32]) {
+    asm volatile(
+        "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,"
+        "%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%32];"
+        : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]), "=r"(v[4]), "=r"(v[5]), "=r"(v[6]), "=r"(v[7]), "=r"(v[8]),
+          "=r"(v[9]), "=r"(v[10]), "=r"(v[11]), "=r"(v[12]), "=r"(v[13]), "=r"(v[14]), "=r"(v[15]), "=r"(v[16]),
+          "=r"(v[17]), "=r"(v[18]), "=r"(v[19]), "=r"(v[20]), "=r"(v[21]), "=r"(v[22]), "=r"(v[23]), "=r"(v[24]),
+          "=r"(v[25]), "=r"(v[26]), "=r"(v[27]), "=r"(v[28]), "=r"(v[29]), "=r"(v[30]), "=r"(v[31])
+        : "r"(taddr));
+}
+// The loads' registers pass through the wait, so that no use of them moves in front of it.
+__device__ __forceinline__ void pa_wait_ld(uint32_t (&v)[32]) {
+    asm volatile("tcgen05.wait::ld.sync.aligned;"
+                 : "+r"(v[0]), "+r"(v[1]), "+r"(v[2]), "+r"(v[3]), "+r"(v[4]), "+r"(v[5]), "+r"(v[6]), "+r"(v[7]),
+                   "+r"(v[8]), "+r"(v[9]), "+r"(v[10]), "+r"(v[11]), "+r"(v[12]), "+r"(v[13]), "+r"(v[14]),
+                   "+r"(v[15]), "+r"(v[16]), "+r"(v[17]), "+r"(v[18]), "+r"(v[19]), "+r"(v[20]), "+r"(v[21]),
+                   "+r"(v[22]), "+r"(v[23]), "+r"(v[24]), "+r"(v[25]), "+r"(v[26]), "+r"(v[27]), "+r"(v[28]),
+                   "+r"(v[29]), "+r"(v[30]), "+r"(v[31])
+                 :
+                 : "memory");
+}
+__device__ __forceinline__ void pa_st32(uint32_t taddr, const uint32_t (&v)[32]) {
+    asm volatile(
+        "tcgen05.st.sync.aligned.32x32b.x32.b32 [%32], {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,"
+        "%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31};" ::"r"(v[0]),
+        "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7]), "r"(v[8]), "r"(v[9]), "r"(v[10]),
+        "r"(v[11]), "r"(v[12]), "r"(v[13]), "r"(v[14]), "r"(v[15]), "r"(v[16]), "r"(v[17]), "r"(v[18]), "r"(v[19]),
+        "r"(v[20]), "r"(v[21]), "r"(v[22]), "r"(v[23]), "r"(v[24]), "r"(v[25]), "r"(v[26]), "r"(v[27]), "r"(v[28]),
+        "r"(v[29]), "r"(v[30]), "r"(v[31]), "r"(taddr)
+        : "memory");
+}
+__device__ __forceinline__ void pa_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
+__device__ __forceinline__ float ex2(float x) {
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+template <class T> __device__ __forceinline__ uint32_t pa_pack(float lo, float hi);
+template <> __device__ __forceinline__ uint32_t pa_pack<__half>(float lo, float hi) {
+    const __half2 h = __floats2half2_rn(lo, hi);
+    return *reinterpret_cast<const uint32_t*>(&h);
+}
+template <> __device__ __forceinline__ uint32_t pa_pack<__nv_bfloat16>(float lo, float hi) {
+    const __nv_bfloat162 h = __floats2bfloat162_rn(lo, hi);
+    return *reinterpret_cast<const uint32_t*>(&h);
+}
+
+template <int HD>
+constexpr int pa_stages() { return HD == 128 ? 4 : 8; }
+template <int HD>
+constexpr size_t pa_smem(int n_req) {
+    return (size_t)2 * (HD / 64) * kPaHalf + (size_t)pa_stages<HD>() * (HD / 64) * kPaHalf + sizeof(PaCtl) +
+           ((size_t)n_req + 1) * 4 + 1024;
+}
+
+// MOD: capped or biased scores, or a scale that is not positive (then the maximum is not that of q.k).
+template <class T, int HD, bool MOD>
+__global__ void __launch_bounds__(kPaThreads, 1) k_pattn(const __grid_constant__ PaArgs p) {
+    constexpr int NST = pa_stages<HD>();
+    constexpr int NH = HD / 64;                 // 64-element halves of a row
+    constexpr uint32_t TILE = NH * kPaHalf;     // bytes of a Q, K or V tile
+    constexpr bool BF = sizeof(T) == 2 && !std::is_same<T, __half>::value;
+    // fp16 weights are kept 2^6 above the running maximum's scale (at most 2^14 with the 2^8 slack), so that small
+    // ones stay in the type's normal range
+    constexpr float kShift = BF ? 0.f : 6.f;
+    constexpr float kSlack = 8.f;
+    extern __shared__ uint8_t raw[];
+    uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(raw) + 1023) & ~(uintptr_t)1023);
+    const uint32_t qs = smem_u32(smem), kvs = qs + 2 * TILE;
+    PaCtl* ctl = reinterpret_cast<PaCtl*>(smem + (2 + NST) * TILE);
+    int* ustart = reinterpret_cast<int*>(ctl + 1);
+    const sd_attn_args& a = p.a;
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+
+    if (tid == 0) {
+        mbar_init(&ctl->qfull, 1);
+        mbar_init(&ctl->qempty, 1);
+        for (int i = 0; i < NST; ++i) {
+            mbar_init(&ctl->full[i], 1);
+            mbar_init(&ctl->empty[i], 2);
+            mbar_init(&ctl->fixed[i], 1);
+        }
+        for (int i = 0; i < 2; ++i) {
+            mbar_init(&ctl->sfull[i], 1);
+            mbar_init(&ctl->pready[i], 128);
+            mbar_init(&ctl->ofull[i], 1);
+        }
+        mbar_init(&ctl->mready, 128);
+        mbar_init(&ctl->mdone, 128);
+        mbar_init(&ctl->done, 1);
+        ctl->abort = 0;
+        fence_mbar_init();
+    }
+    if (warp == 9) {
+        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], 512;" ::"r"(smem_u32(&ctl->tmem)) : "memory");
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+    }
+    // units (row tiles x chunks) of each request: exclusive sums
+    {
+        const int n = a.n_req, per = (n + kPaThreads - 1) / kPaThreads;
+        const int b0 = min(n, tid * per), b1 = min(n, b0 + per);
+        int sum = 0;
+        bool bad = false;
+        for (int b = b0; b < b1; ++b) {
+            const int rows = pa_rows(a, b), u = rows > 0 ? pa_tiles(p, rows) * pa_chunks(p, pa_kv(a, b), pa_inline(p, rows)) : 0;
+            bad |= a.q_len[b] > a.max_q || a.q_len[b] < 0 || a.kv_len[b] > a.max_kv || a.kv_len[b] < 0 || a.q_start[b] < 0 ||
+                   rows < pa_q(a, b);
+            ustart[b] = u;
+            sum += u;
+        }
+        if (bad && blockIdx.x == 0) set_dev_error(p.err, DEV_ERR_BAD_ARG);
+        int incl = sum;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+            const int v = __shfl_up_sync(0xffffffffu, incl, o);
+            if (lane >= o) incl += v;
+        }
+        if (lane == 31) ctl->wsum[warp] = incl;
+        __syncthreads();
+        int before = 0;
+        for (int w = 0; w < warp; ++w) before += ctl->wsum[w];
+        int run = before + incl - sum;
+        for (int b = b0; b < b1; ++b) {
+            const int u = ustart[b];
+            ustart[b] = run;
+            run += u;
+        }
+        if (tid == kPaThreads - 1) ustart[n] = before + incl;
+    }
+    pa_fence_before();
+    __syncthreads();
+    pa_fence_after();
+    const uint32_t tmem = ctl->tmem;
+    const int n_items = (p.cp * p.n_pt + ustart[a.n_req]) * a.pool.n_kv_heads;
+    const int ps = a.pool.page_size, G = p.G;
+
+    if (warp == 8) {
+        // ---------------- TMA ----------------
+        uint32_t pos = 0;
+        int nq = 0;
+        const int box = min(ps, kPaKeys), npg = kPaKeys / box;  // pages per key tile
+        const uint32_t page_bytes = (uint32_t)box * 128u * NH;
+        bool ok = true;
+        for (int i = blockIdx.x; i < n_items && ok; i += gridDim.x) {
+            PaItem it;
+            if (!pa_item(p, ustart, i, it) || it.n == 0) continue;
+            if (nq > 0 && !pa_wait_warp(&ctl->qempty, (nq - 1) & 1, ctl, p.err, DEV_ERR_EMPTY_WAIT)) break;
+            if (lane == 0) {
+                const int nslot = it.pair ? 2 : 1;
+                mbar_arrive_expect_tx(&ctl->qfull, (uint32_t)(nslot * NH * p.TPT * G * 128));
+                for (int s = 0; s < nslot; ++s)
+                    for (int h = 0; h < NH; ++h)
+                        tma_3d(qs + s * TILE + h * kPaHalf, &p.tq, h * 64, it.kvh * G, it.tok0 + s * p.TPT, &ctl->qfull);
+            }
+            ++nq;
+            for (int t = 0; t < it.n; ++t) {
+                const PaTile kt = pa_tile(p, it, it.v0 + t);
+                // lane g < npg: page g of the tile
+                const int key = kt.k0 + lane * box;
+                const bool want = lane < npg && key < kt.hi && key + box > kt.lo;
+                int page = -1;
+                if (want) page = kt.prefix ? a.prefix_table[key / ps] : a.table[(size_t)it.b * a.table_ld + key / ps];
+                const bool have = want && page >= 0 && page < a.pool.n_pages;
+                if (want && !have) set_dev_error(p.err, DEV_ERR_BAD_ARG);
+                const uint32_t got = __ballot_sync(0xffffffffu, have);
+                uint32_t mask = 0;  // bits of 16-key groups
+                for (int g = 0; g < npg; ++g)
+                    if (got >> g & 1) mask |= ((1u << (box / 16)) - 1) << (g * (box / 16));
+#pragma unroll
+                for (int kv = 0; kv < 2; ++kv) {
+                    const int st = pos % NST;
+                    if (pos >= NST && !pa_wait_warp(&ctl->empty[st], (pos / NST - 1) & 1, ctl, p.err, DEV_ERR_EMPTY_WAIT)) {
+                        ok = false;
+                        break;
+                    }
+                    if (lane == 0) {
+                        if (kv == 0) ctl->okmask[(pos >> 1) & 15] = mask;
+                        mbar_arrive_expect_tx(&ctl->full[st], __popc(got) * page_bytes);
+                    }
+                    __syncwarp();
+                    if (have)
+                        for (int h = 0; h < NH; ++h)
+                            tma_4d(kvs + st * TILE + h * kPaHalf + lane * box * 128, kv ? &p.tv : &p.tk, h * 64, key & (ps - 1), it.kvh,
+                                   page, &ctl->full[st]);
+                    ++pos;
+                }
+                if (!ok) break;
+            }
+        }
+        // no copy may still be landing when the CTA exits
+        for (uint32_t q = pos > NST ? pos - NST : 0; q < pos; ++q) mbar_wait(&ctl->full[q % NST], (q / NST) & 1);
+        if (nq > 0) mbar_wait(&ctl->qfull, (nq - 1) & 1);
+    } else if (warp == 9) {
+        // ---------------- MMA issue ----------------
+        if (lane == 0) {
+            constexpr uint32_t id_s = idesc_f16(BF, kPaKeys, false), id_o = idesc_f16(BF, HD, true);
+            uint32_t pos = 0, fixes = 0, np[2] = {0, 0};
+            int nq = 0;
+            bool ok = true;
+            auto wait_k = [&](uint32_t q) {
+                ok = ok && pa_wait(&ctl->full[q % NST], (q / NST) & 1, ctl, p.err, DEV_ERR_FULL_WAIT);
+                pa_fence_after();
+            };
+            auto score = [&](int slot, int qt, uint32_t q) {
+                const uint32_t qa = qs + qt * TILE, ka = kvs + (q % NST) * TILE;
+#pragma unroll
+                for (int ks = 0; ks < HD / 16; ++ks)
+                    mma_ss(tmem + slot * 128, sw128_desc(qa + (ks >> 2) * kPaHalf + (ks & 3) * 32, 16, 1024),
+                           sw128_desc(ka + (ks >> 2) * kPaHalf + (ks & 3) * 32, 16, 1024), id_s, ks > 0);
+                pa_commit(&ctl->sfull[slot]);
+            };
+            auto wait_p = [&](int slot) {
+                ok = ok && pa_wait(&ctl->pready[slot], np[slot] & 1, ctl, p.err, DEV_ERR_FULL_WAIT);
+                ++np[slot];
+                pa_fence_after();
+            };
+            auto wait_v = [&](const PaItem& it, int t, uint32_t q) {
+                wait_k(q);
+                if (!ok) return;
+                const PaTile kt = pa_tile(p, it, it.v0 + t);
+                const int st = q % NST;
+                if (kt.k0 < kt.lo || kt.k0 + kPaKeys > kt.hi || ctl->okmask[(q >> 1) & 15] != 0xFFu) {
+                    ok = pa_wait(&ctl->fixed[st], fixes >> st & 1, ctl, p.err, DEV_ERR_FULL_WAIT);
+                    fixes ^= 1u << st;
+                }
+            };
+            auto value = [&](int slot, bool acc, uint32_t q) {
+                const uint32_t va = kvs + (q % NST) * TILE;
+#pragma unroll
+                for (int ks = 0; ks < kPaKeys / 16; ++ks)
+                    mma_ts(tmem + 256 + slot * HD, tmem + slot * 128 + ks * 8, sw128_desc(va + ks * 2048, kPaHalf, 1024), id_o,
+                           acc || ks > 0);
+                pa_commit(&ctl->ofull[slot]);
+            };
+            for (int i = blockIdx.x; i < n_items && ok; i += gridDim.x) {
+                PaItem it;
+                if (!pa_item(p, ustart, i, it) || it.n == 0) continue;
+                ok = pa_wait(&ctl->qfull, nq & 1, ctl, p.err, DEV_ERR_FULL_WAIT);
+                ++nq;
+                const uint32_t k0 = pos;
+                const int n = it.n;
+                pos += 2 * n;
+                wait_k(k0);
+                if (!ok) break;
+                if (it.pair) {
+                    score(0, 0, k0);
+                    score(1, 1, k0);
+                    pa_commit(&ctl->empty[k0 % NST]);
+                    if (n == 1) pa_commit(&ctl->qempty);
+                    for (int t = 0; t < n && ok; ++t) {
+                        const uint32_t v = k0 + 2 * t + 1, kn = v + 1;
+                        wait_v(it, t, v);
+                        if (ok) wait_p(0);
+                        if (!ok) break;
+                        value(0, t > 0, v);
+                        if (t + 1 < n) {
+                            wait_k(kn);
+                            if (!ok) break;
+                            score(0, 0, kn);
+                        }
+                        wait_p(1);
+                        if (!ok) break;
+                        value(1, t > 0, v);
+                        pa_commit(&ctl->empty[v % NST]);
+                        if (t + 1 < n) {
+                            score(1, 1, kn);
+                            pa_commit(&ctl->empty[kn % NST]);
+                            if (t + 2 == n) pa_commit(&ctl->qempty);
+                        }
+                    }
+                } else {
+                    score(0, 0, k0);
+                    pa_commit(&ctl->empty[k0 % NST]);
+                    if (n > 1) {
+                        wait_k(k0 + 2);
+                        if (!ok) break;
+                        score(1, 0, k0 + 2);
+                        pa_commit(&ctl->empty[(k0 + 2) % NST]);
+                    }
+                    if (n <= 2) pa_commit(&ctl->qempty);
+                    for (int t = 0; t < n && ok; ++t) {
+                        const uint32_t v = k0 + 2 * t + 1, kn = v + 3;
+                        wait_v(it, t, v);
+                        if (ok) wait_p(t & 1);
+                        if (!ok) break;
+                        value(t & 1, t > 1, v);
+                        pa_commit(&ctl->empty[v % NST]);
+                        if (t + 2 < n) {
+                            wait_k(kn);
+                            if (!ok) break;
+                            score(t & 1, 0, kn);
+                            pa_commit(&ctl->empty[kn % NST]);
+                            if (t + 3 == n) pa_commit(&ctl->qempty);
+                        }
+                    }
+                }
+            }
+            // every MMA issued above has completed before the tensor memory is released
+            pa_commit(&ctl->done);
+            if (!mbar_wait(&ctl->done, 0)) set_dev_error(p.err, DEV_ERR_FULL_WAIT);
+        }
+        __syncwarp();
+    } else if (warp == 10) {
+        // ---------------- V rows that no row of the item may see become zero ----------------
+        uint32_t pos = 0;
+        bool ok = true;
+        for (int i = blockIdx.x; i < n_items && ok; i += gridDim.x) {
+            PaItem it;
+            if (!pa_item(p, ustart, i, it) || it.n == 0) continue;
+            for (int t = 0; t < it.n && ok; ++t) {
+                const PaTile kt = pa_tile(p, it, it.v0 + t);
+#pragma unroll
+                for (int kv = 0; kv < 2; ++kv) {
+                    const int st = pos % NST;
+                    ok = ok && pa_wait_warp(&ctl->full[st], (pos / NST) & 1, ctl, p.err, DEV_ERR_FULL_WAIT);
+                    if (!ok) break;
+                    if (kv) {
+                        const uint32_t mask = ctl->okmask[(pos >> 1) & 15];
+                        if (kt.k0 < kt.lo || kt.k0 + kPaKeys > kt.hi || mask != 0xFFu) {
+                            // 8 lanes a row (16 bytes each of 128), 4 rows at a time
+                            for (int r = lane >> 3; r < kPaKeys; r += 4)
+                                if (kt.k0 + r < kt.lo || kt.k0 + r >= kt.hi || !(mask >> (r >> 4) & 1))
+                                    for (int h = 0; h < NH; ++h)
+                                        asm volatile("st.shared.v4.u32 [%0], {%1, %1, %1, %1};" ::"r"(
+                                                         kvs + st * TILE + h * kPaHalf + r * 128 + (lane & 7) * 16),
+                                                     "r"(0)
+                                                     : "memory");
+                            asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+                            __syncwarp();
+                            if (lane == 0) mbar_arrive(&ctl->fixed[st]);
+                        }
+                    }
+                    if (lane == 0) mbar_arrive(&ctl->empty[st]);
+                    ++pos;
+                }
+            }
+        }
+    } else if (warp < 8) {
+        // ---------------- softmax: thread = row of its slot ----------------
+        const int slot = warp >> 2, row = tid & 127;
+        const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;
+        const uint32_t ts = tmem + lanes + slot * 128, to = tmem + lanes + 256 + slot * HD;
+        const int row_tok = row / G, row_head = row - row_tok * G;
+        const float kLog2e = 1.4426950408889634f;
+        const float sc2 = a.scale * kLog2e;
+        // capped: cap log2e tanh(x) with x = scale s / cap, as cap log2e (1 - 2 / (1 + 2^(2 log2e x)))
+        const float cap2 = a.softcap * kLog2e, xs = a.softcap > 0.f ? 2.f * kLog2e * a.scale / a.softcap : 0.f;
+        uint32_t ns = 0, no = 0, nm = 0, tiles = 0;
+        bool ok = true;
+        for (int i = blockIdx.x; i < n_items && ok; i += gridDim.x) {
+            PaItem it;
+            if (!pa_item(p, ustart, i, it)) continue;
+            const int tok = it.tok0 + (it.pair ? slot * p.TPT : 0) + row_tok;
+            const int head = it.kvh * G + row_head;
+            const bool live = row_tok < p.TPT && tok < it.tok0 + it.ntok;
+            // the row's own position, and its visible keys in the prefix and in its own positions
+            int own = -1;
+            if (live) {
+                if (it.b >= 0) {
+                    own = it.base + (tok - it.q0);
+                } else {
+                    own = 0;
+                    if (a.window > 0 || a.alibi) {
+                        const int b = pa_request(a, tok);
+                        own = pa_kv(a, b) - pa_q(a, b) + (tok - a.q_start[b]);
+                    }
+                }
+            }
+            const int P = a.prefix_len, W = a.window;
+            const bool seeing = live && own >= 0;
+            const int lo_o = W > 0 ? max(0, own + 1 - W) : 0, hi_o = seeing ? own + 1 : 0;
+            const int lo_p = W > 0 ? max(0, P + own + 1 - W) : 0, hi_p = seeing ? P : 0;
+            const float slope = MOD && a.alibi && live ? a.alibi[head] * kLog2e : 0.f;
+            float m = -INFINITY, l = 0.f;
+            const int step = it.pair ? 1 : 2;
+            bool first = true;
+            for (int t = it.pair ? 0 : slot; t < it.n; t += step) {
+                const PaTile kt = pa_tile(p, it, it.v0 + t);
+                const int lo = (kt.prefix ? lo_p : lo_o) - kt.k0, hi = (kt.prefix ? hi_p : hi_o) - kt.k0;
+                ok = pa_wait_warp(&ctl->sfull[slot], ns & 1, ctl, p.err, DEV_ERR_FULL_WAIT);
+                ++ns;
+                if (!ok) break;
+                pa_fence_after();
+                uint32_t y[4][32];
+#pragma unroll
+                for (int c = 0; c < 4; ++c) pa_ld32(ts + c * 32, y[c]);
+#pragma unroll
+                for (int c = 0; c < 4; ++c) pa_wait_ld(y[c]);
+                if (MOD) {
+                    const float bias = kt.prefix ? slope * (float)(P + own - kt.k0) : slope * (float)(own - kt.k0);
+#pragma unroll
+                    for (int c = 0; c < 4; ++c)
+#pragma unroll
+                        for (int e = 0; e < 32; ++e) {
+                            float s = __uint_as_float(y[c][e]);
+                            if (a.softcap > 0.f) {
+                                s = fmaf(__fdividef(-2.f, 1.f + ex2(s * xs)), cap2, cap2);
+                            } else {
+                                s *= sc2;
+                            }
+                            s += fmaf(slope, (float)(c * 32 + e), -bias);
+                            y[c][e] = __float_as_uint(s);
+                        }
+                }
+                const uint32_t mask = *(volatile uint32_t*)&ctl->okmask[(tiles + t) & 15];
+                if (!__all_sync(0xffffffffu, lo <= 0 && hi >= kPaKeys && mask == 0xFFu)) {
+#pragma unroll
+                    for (int c = 0; c < 4; ++c)
+#pragma unroll
+                        for (int e = 0; e < 32; ++e) {
+                            const int k = c * 32 + e;
+                            if (!(k >= lo && k < hi && (mask >> (k >> 4) & 1))) y[c][e] = 0xff800000u;  // -infinity
+                        }
+                }
+                float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll
+                for (int c = 0; c < 4; ++c)
+#pragma unroll
+                    for (int e = 0; e < 32; ++e) mx[e & 3] = fmaxf(mx[e & 3], __uint_as_float(y[c][e]));
+                float top = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3]));
+                if (!MOD) top *= sc2;
+                float factor = 1.f;
+                if (top > m + kSlack || (m == -INFINITY && top != -INFINITY)) {
+                    factor = ex2(m - top);  // 0 from a maximum of -infinity
+                    m = top;
+                }
+                l *= factor;
+                if (__any_sync(0xffffffffu, factor != 1.f) && !first) {
+                    // O of the tiles so far refers to the old maximum
+                    ok = pa_wait_warp(&ctl->ofull[slot], (no - 1) & 1, ctl, p.err, DEV_ERR_FULL_WAIT);
+                    if (!ok) break;
+                    pa_fence_after();
+#pragma unroll
+                    for (int c = 0; c < HD / 32; ++c) {
+                        uint32_t o[32];
+                        pa_ld32(to + c * 32, o);
+                        pa_wait_ld(o);
+#pragma unroll
+                        for (int e = 0; e < 32; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * factor);
+                        pa_st32(to + c * 32, o);
+                    }
+                }
+                const float ref = (m == -INFINITY ? 0.f : m) - kShift;
+                float sum[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+                for (int h = 0; h < 2; ++h) {
+                    uint32_t pk[32];
+#pragma unroll
+                    for (int e = 0; e < 32; ++e) {
+                        const int c = h * 2 + (e >> 4), x = (e & 15) * 2;
+                        const float s0 = __uint_as_float(y[c][x]), s1 = __uint_as_float(y[c][x + 1]);
+                        const float p0 = ex2(MOD ? s0 - ref : fmaf(s0, sc2, -ref)), p1 = ex2(MOD ? s1 - ref : fmaf(s1, sc2, -ref));
+                        sum[(e & 1) * 2] += p0;
+                        sum[(e & 1) * 2 + 1] += p1;
+                        pk[e] = pa_pack<T>(p0, p1);
+                    }
+                    pa_st32(ts + h * 32, pk);
+                }
+                l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
+                pa_wait_st();
+                pa_fence_before();
+                mbar_arrive(&ctl->pready[slot]);
+                ++no;
+                first = false;
+            }
+            if (!ok) break;
+            tiles += it.n;
+            // ---- the item's result ----
+            if (!first) {
+                ok = pa_wait_warp(&ctl->ofull[slot], (no - 1) & 1, ctl, p.err, DEV_ERR_FULL_WAIT);
+                if (!ok) break;
+                pa_fence_after();
+            }
+            float f0 = 1.f, f1 = 0.f;
+            const bool merge = !it.pair && it.n > 1;
+            if (merge) {
+                if (slot == 1) {
+                    ctl->ml1[row] = make_float2(m, l);
+                    pa_fence_before();
+                    mbar_arrive(&ctl->mready);
+                } else {
+                    ok = pa_wait_warp(&ctl->mready, nm & 1, ctl, p.err, DEV_ERR_FULL_WAIT);
+                    if (!ok) break;
+                    pa_fence_after();
+                    const float2 other = ctl->ml1[row];
+                    const float mm = fmaxf(m, other.x), mr = mm == -INFINITY ? 0.f : mm;
+                    f0 = ex2(m - mr);
+                    f1 = ex2(other.x - mr);
+                    m = mm;
+                    l = l * f0 + other.y * f1;
+                }
+            }
+            if (it.pair || slot == 0) {
+                const size_t orow = (size_t)tok * a.n_heads + head;
+                const size_t prow = (size_t)it.split * a.n_tokens * a.n_heads + orow;
+                const float inv = l > 0.f ? 1.f / l : (l == 0.f ? 0.f : l);  // NaN stays NaN
+#pragma unroll 1
+                for (int c = 0; c < HD / 32; ++c) {
+                    uint32_t o[32];
+                    if (it.n > 0) {
+                        pa_ld32(to + c * 32, o);
+                        pa_wait_ld(o);
+                        if (merge) {
+                            uint32_t o1[32];
+                            pa_ld32(to + HD + c * 32, o1);
+                            pa_wait_ld(o1);
+#pragma unroll
+                            for (int e = 0; e < 32; ++e)
+                                o[e] = __float_as_uint(__uint_as_float(o[e]) * f0 + __uint_as_float(o1[e]) * f1);
+                        }
+                    } else {
+#pragma unroll
+                        for (int e = 0; e < 32; ++e) o[e] = 0u;
+                    }
+                    if (!live) continue;
+                    if (it.direct) {
+                        uint4* dst = reinterpret_cast<uint4*>(static_cast<T*>(a.out) + (size_t)tok * a.out_ld + (size_t)head * a.out_head + c * 32);
+                        uint32_t pk[16];
+#pragma unroll
+                        for (int e = 0; e < 16; ++e)
+                            pk[e] = pa_pack<T>(__uint_as_float(o[2 * e]) * inv, __uint_as_float(o[2 * e + 1]) * inv);
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) dst[e] = make_uint4(pk[4 * e], pk[4 * e + 1], pk[4 * e + 2], pk[4 * e + 3]);
+                    } else {
+                        float4* dst = reinterpret_cast<float4*>(p.acc + prow * HD + c * 32);
+#pragma unroll
+                        for (int e = 0; e < 8; ++e)
+                            dst[e] = make_float4(__uint_as_float(o[4 * e]), __uint_as_float(o[4 * e + 1]), __uint_as_float(o[4 * e + 2]),
+                                                 __uint_as_float(o[4 * e + 3]));
+                    }
+                }
+                if (!it.direct && live) p.ml[prow] = make_float2(m, l);
+            }
+            if (merge) {
+                if (slot == 0) {
+                    pa_fence_before();
+                    mbar_arrive(&ctl->mdone);
+                } else {
+                    ok = pa_wait_warp(&ctl->mdone, nm & 1, ctl, p.err, DEV_ERR_FULL_WAIT);
+                    if (!ok) break;
+                }
+                ++nm;
+            }
+        }
+    }
+    pa_fence_before();
+    __syncthreads();
+    pa_fence_after();
+    if (warp == 9) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, 512;" ::"r"(tmem) : "memory");
+}
+
+// Joins the states that the items of a row left: o = sum_i 2^(m_i - M) O_i / sum_i 2^(m_i - M) l_i, in split order.
+// One warp per (token, head), lane = 4 (head_dim 128) or 2 dims.
+template <class T, int HD>
+__global__ void __launch_bounds__(256) k_pattn_combine(const __grid_constant__ PaArgs p) {
+    constexpr int V = HD / 32;
+    const sd_attn_args& a = p.a;
+    const int tok = blockIdx.x, head = blockIdx.y * 8 + (threadIdx.x >> 5), lane = threadIdx.x & 31;
+    if (head >= a.n_heads) return;
+    const int b = pa_request(a, tok), t = tok - a.q_start[b], rows = pa_rows(a, b);
+    if (t < 0 || t >= rows) return;
+    const int kv = pa_kv(a, b);
+    const bool inl = pa_inline(p, rows);
+    const int chunks = pa_chunks(p, kv, inl);
+    if (chunks == 1 && (a.prefix_len == 0 || inl)) return;  // written by its item
+    const bool seeing = kv - pa_q(a, b) + t >= 0;
+    const int s0 = inl ? p.cp : 0, s1 = seeing ? p.cp + chunks : s0;
+    const size_t row = (size_t)tok * a.n_heads + head, ld = (size_t)a.n_tokens * a.n_heads;
+    float M = -INFINITY;
+    for (int s = s0 + lane; s < s1; s += 32) M = fmaxf(M, p.ml[s * ld + row].x);
+    M = warp_max(M);
+    if (M == -INFINITY) M = 0.f;
+    float L = 0.f, o[V];
+#pragma unroll
+    for (int e = 0; e < V; ++e) o[e] = 0.f;
+    for (int s = s0; s < s1; ++s) {
+        const float2 ml = p.ml[s * ld + row];
+        if (ml.y == 0.f) continue;
+        const float f = ex2(ml.x - M);
+        L = fmaf(ml.y, f, L);
+        const float* acc = p.acc + (s * ld + row) * HD + lane * V;
+#pragma unroll
+        for (int e = 0; e < V; ++e) o[e] = fmaf(acc[e], f, o[e]);
+    }
+    const float inv = L > 0.f ? 1.f / L : (L == 0.f ? 0.f : L);
+    uint32_t* dst = reinterpret_cast<uint32_t*>(static_cast<T*>(a.out) + (size_t)tok * a.out_ld + (size_t)head * a.out_head + lane * V);
+#pragma unroll
+    for (int e = 0; e < V / 2; ++e) dst[e] = pa_pack<T>(o[2 * e] * inv, o[2 * e + 1] * inv);
+}
+
+// ---------------------------------------------------------------------------------------------
+// Host side
+// ---------------------------------------------------------------------------------------------
+using EncodeTiled = CUresult (*)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*, const cuuint64_t*,
+                                 const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave, CUtensorMapSwizzle,
+                                 CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+
+EncodeTiled encode_tiled() {
+    static EncodeTiled fn = [] {
+        void* f = nullptr;
+        cudaDriverEntryPointQueryResult q;
+        if (cudaGetDriverEntryPointByVersion("cuTensorMapEncodeTiled", &f, 12000, cudaEnableDefault, &q) != cudaSuccess ||
+            q != cudaDriverEntryPointSuccess)
+            f = nullptr;
+        return reinterpret_cast<EncodeTiled>(f);
+    }();
+    return fn;
+}
+
+// What TMA and 16-byte accesses need; other calls take the general kernel.
+bool tc_able(const sd_attn_args& a) {
+    const sd_kv_pool& k = a.pool;
+    auto al = [](const void* q) { return (reinterpret_cast<uintptr_t>(q) & 15) == 0; };
+    auto st = [](int64_t s) { return s % 8 == 0 && s < (1ll << 38); };
+    return (k.head_dim == 64 || k.head_dim == 128) && al(k.k) && al(k.v) && al(a.q) && al(a.out) && st(k.page_stride) &&
+           st(k.pos_stride) && st(k.head_stride) && st(a.q_ld) && st(a.q_head) && st(a.out_ld) && st(a.out_head);
+}
+
+// How the work of a call is cut: depends on what the host knows only (counts and bounds), so a request's split
+// does not depend on the other requests' lengths.
+void pa_plan(const sd_attn_args& a, int sms, PaArgs* p) {
+    p->a = a;
+    p->G = a.n_heads / a.pool.n_kv_heads;
+    p->TPT = 128 / p->G;
+    const int n_kv = a.pool.n_kv_heads, pair = 2 * p->TPT;
+    p->np = (a.prefix_len + kPaKeys - 1) / kPaKeys;
+    const int own = (a.max_kv + kPaKeys - 1) / kPaKeys + (a.max_q > pair ? p->np : 0);
+    // own items: aim at four per SM, but not below 8 key tiles (an item costs about one tile to start and to join)
+    // over the tiles that an item can see through the window; if those fit one chunk, nothing is cut
+    const long long units = (long long)n_kv * std::max<long long>(a.n_req, a.n_tokens / pair);
+    const int seen = a.window > 0 ? (int)std::min<long long>(own, ((long long)a.window + std::min(a.max_q, pair)) / kPaKeys + 2) : own;
+    long long ct = std::max<long long>(8, (units * seen + 4LL * sms - 1) / (4LL * sms));
+    p->ct_own = ct >= seen ? std::max(own, 1) : (int)ct;
+    // prefix items: the same over the tokens' row tiles
+    p->n_pt = p->np ? (a.n_tokens + pair - 1) / pair : 0;
+    p->ct_pre = 1;
+    p->cp = 0;
+    if (p->np) {
+        ct = std::max<long long>(4, ((long long)n_kv * p->n_pt * p->np + 2LL * sms - 1) / (2LL * sms));
+        p->ct_pre = (int)std::min<long long>(p->np, ct);
+        p->cp = (p->np + p->ct_pre - 1) / p->ct_pre;
+    }
+}
+
+int pa_splits(const PaArgs& p) {
+    const sd_attn_args& a = p.a;
+    const int own = (a.max_kv + kPaKeys - 1) / kPaKeys + (p.np && a.max_q > 2 * p.TPT ? p.np : 0);
+    const int chunks = std::max(1, (own + p.ct_own - 1) / p.ct_own);
+    return chunks == 1 && p.np == 0 ? 0 : p.cp + chunks;
+}
+
+size_t pa_workspace(const PaArgs& p) {
+    const size_t rows = (size_t)pa_splits(p) * p.a.n_tokens * p.a.n_heads;
+    return rows * ((size_t)p.a.pool.head_dim * 4 + 8);
+}
+
+int encode(CUtensorMap* m, bool bf16, int rank, const void* base, const cuuint64_t* dims, const cuuint64_t* strides,
+           const cuuint32_t* box) {
+    const cuuint32_t ones[5] = {1, 1, 1, 1, 1};
+    EncodeTiled fn = encode_tiled();
+    if (!fn) return fail(SD_ERR_UNSUPPORTED, "cuTensorMapEncodeTiled is not available");
+    const CUresult r = fn(m, bf16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, rank, const_cast<void*>(base),
+                          dims, strides, box, ones, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+                          CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    return r == CUDA_SUCCESS ? SD_OK : fail(SD_ERR_INVALID, "attention: tensor map refused (%d)", (int)r);
+}
+
+static_assert(pa_smem<128>(SD_PAGES_MAX_REQ) <= 232448, "the largest batch fits the shared memory");
+
+template <class T, int HD, bool MOD>
+int launch_tc(const PaArgs& p, int grid, cudaStream_t st) {
+    const size_t smem = pa_smem<HD>(p.a.n_req);
+    cudaError_t e = cudaFuncSetAttribute(k_pattn<T, HD, MOD>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+    if (e != cudaSuccess) return cuda_fail(e, "attention attributes");
+    k_pattn<T, HD, MOD><<<grid, kPaThreads, smem, st>>>(p);
+    if ((e = cudaGetLastError()) != cudaSuccess) return cuda_fail(e, "attention");
+    if (pa_splits(p) > 0) {
+        k_pattn_combine<T, HD><<<dim3(p.a.n_tokens, (p.a.n_heads + 7) / 8), 256, 0, st>>>(p);
+        if ((e = cudaGetLastError()) != cudaSuccess) return cuda_fail(e, "attention combine");
+    }
+    return SD_OK;
+}
+
+int run_tc(const sd_attn_args& a, int dev, cudaStream_t st) {
+    PaArgs p{};
+    pa_plan(a, device_sm_count(dev), &p);
+    const size_t need = pa_workspace(p);
+    if (need > 0 && (!a.workspace || a.workspace_bytes < need || (reinterpret_cast<uintptr_t>(a.workspace) & 255)))
+        return fail(SD_ERR_INVALID, "sd_attention_dev: %zu bytes of 256-byte aligned workspace needed", need);
+    const size_t rows = (size_t)pa_splits(p) * a.n_tokens * a.n_heads;
+    p.acc = static_cast<float*>(a.workspace);
+    p.ml = reinterpret_cast<float2*>(p.acc + rows * a.pool.head_dim);
+    p.err = device_error_word(dev);
+    const sd_kv_pool& k = a.pool;
+    const bool bf = k.dtype == SD_BF16;
+    const cuuint64_t hd = k.head_dim;
+    {
+        const cuuint64_t dims[3] = {hd, (cuuint64_t)a.n_heads, (cuuint64_t)a.n_tokens};
+        const cuuint64_t strides[2] = {(cuuint64_t)a.q_head * 2, (cuuint64_t)a.q_ld * 2};
+        const cuuint32_t box[3] = {64, (cuuint32_t)p.G, (cuuint32_t)p.TPT};
+        const int rc = encode(&p.tq, bf, 3, a.q, dims, strides, box);
+        if (rc) return rc;
+    }
+    for (int i = 0; i < 2; ++i) {
+        const cuuint64_t dims[4] = {hd, (cuuint64_t)k.page_size, (cuuint64_t)k.n_kv_heads, (cuuint64_t)k.n_pages};
+        const cuuint64_t strides[3] = {(cuuint64_t)k.pos_stride * 2, (cuuint64_t)k.head_stride * 2, (cuuint64_t)k.page_stride * 2};
+        const cuuint32_t box[4] = {64, (cuuint32_t)std::min(k.page_size, kPaKeys), 1, 1};
+        const int rc = encode(i ? &p.tv : &p.tk, bf, 4, i ? k.v : k.k, dims, strides, box);
+        if (rc) return rc;
+    }
+    const int pair = 2 * p.TPT;
+    const int own = (a.max_kv + kPaKeys - 1) / kPaKeys + (p.np && a.max_q > pair ? p.np : 0);
+    const long long items = (long long)k.n_kv_heads * ((long long)p.cp * p.n_pt + ((long long)a.n_req + a.n_tokens / pair) *
+                                                       std::max(1, (own + p.ct_own - 1) / p.ct_own));
+    if (items > INT32_MAX) return fail(SD_ERR_INVALID, "sd_attention_dev: too many work items");
+    const int grid = (int)std::min<long long>(items, device_sm_count(dev));
+    const bool mod = a.softcap > 0.f || a.alibi || !(a.scale > 0.f);
+    if (bf) {
+        if (k.head_dim == 128) return mod ? launch_tc<__nv_bfloat16, 128, true>(p, grid, st) : launch_tc<__nv_bfloat16, 128, false>(p, grid, st);
+        return mod ? launch_tc<__nv_bfloat16, 64, true>(p, grid, st) : launch_tc<__nv_bfloat16, 64, false>(p, grid, st);
+    }
+    if (k.head_dim == 128) return mod ? launch_tc<__half, 128, true>(p, grid, st) : launch_tc<__half, 128, false>(p, grid, st);
+    return mod ? launch_tc<__half, 64, true>(p, grid, st) : launch_tc<__half, 64, false>(p, grid, st);
+}
+
 int check_attention(const sd_attn_args* a) {
     const char* what = "sd_attention_dev";
     if (!a) return fail(SD_ERR_INVALID, "%s: null arguments", what);
@@ -128,7 +1068,14 @@ int check_attention(const sd_attn_args* a) {
 
 extern "C" {
 
-size_t sd_attention_workspace(const sd_attn_args*) { return 0; }
+size_t sd_attention_workspace(const sd_attn_args* a) {
+    if (check_attention(a) || a->n_tokens == 0 || !tc_able(*a)) return 0;
+    int dev = 0;
+    if (cudaGetDevice(&dev) != cudaSuccess) dev = 0;
+    PaArgs p{};
+    pa_plan(*a, device_sm_count(dev), &p);
+    return pa_workspace(p);
+}
 
 int sd_attention_dev(const sd_attn_args* a, void* stream) {
     clear_error();
@@ -136,6 +1083,7 @@ int sd_attention_dev(const sd_attn_args* a, void* stream) {
     if (rc) return rc;
     if (a->n_tokens == 0) return SD_OK;
     if ((rc = paged_device(a->pool.k, "sd_attention_dev", &dev))) return rc;
+    if (tc_able(*a)) return run_tc(*a, dev, (cudaStream_t)stream);
     const long long rows = (long long)a->n_tokens * a->n_heads;
     if ((rows + 3) / 4 > INT32_MAX) return fail(SD_ERR_INVALID, "sd_attention_dev: too many rows");
     const int grid = (int)((rows + 3) / 4);
