@@ -116,7 +116,7 @@ __global__ void __launch_bounds__(128) k_pattn_general(const sd_attn_args a, int
 // the workspace for k_pattn_combine; others are written by their item.
 //
 // Warps (12): 0-3 softmax of slot 0, 4-7 of slot 1 (thread = row), 8 TMA, 9 MMA issue, 10 zeroes V rows that no row
-// may see (0 x NaN is NaN in the product), 11 idle.  P overwrites S in tensor memory and is the A operand of P V.
+// may see (0 x NaN is NaN in the product), 11 hands out the items.  P overwrites S in tensor memory and is the A operand of P V.
 // The running maximum that O refers to moves only when a row's maximum rises by more than 2^8 (exact: O and the sum
 // refer to the same value), so O is rarely rescaled.  Every wait is bounded in time (sd_common.cuh).
 // ---------------------------------------------------------------------------------------------
@@ -141,6 +141,9 @@ struct PaCtl {
     uint64_t full[8], empty[8], fixed[8];
     uint64_t sfull[2], pready[2], ofull[2];
     uint64_t mready, mdone, done;
+    uint64_t ifull, iempty, claim;  // hand-over of the next item; answer to the claim of another CTA's
+    uint4 claimed;
+    int item;
     uint32_t okmask[16];  // per key tile, in turn: which of its 16-key groups were loaded
     float2 ml1[128];      // slot 1's state at a merge
     uint32_t tmem;
@@ -242,18 +245,20 @@ __device__ __forceinline__ bool pa_item(const PaArgs& p, const int* ustart, int 
     return true;
 }
 
-// Keys [k0, k0 + 128) of virtual tile v of the item, and which of them its rows may see.
+// Keys [k0, k0 + 128) of the item's t-th tile, and which of them its rows may see.  The nearest keys come first: with a
+// distance bias the largest scores then do too, and O keeps its scale (measured at the 2 x 2048-token biased prompts).
 struct PaTile {
     bool prefix;
     int k0, lo, hi;
 };
-__device__ __forceinline__ PaTile pa_tile(const PaArgs& p, const PaItem& it, int v) {
-    PaTile t;
-    t.prefix = v < it.npt;
-    t.k0 = (t.prefix ? v : v - it.npt) * kPaKeys;
-    t.lo = t.prefix ? it.klo_p : it.klo_o;
-    t.hi = t.prefix ? p.a.prefix_len : it.khi_o;
-    return t;
+__device__ __forceinline__ PaTile pa_tile(const PaArgs& p, const PaItem& it, int t) {
+    const int v = it.v0 + it.n - 1 - t;
+    PaTile k;
+    k.prefix = v < it.npt;
+    k.k0 = (k.prefix ? v : v - it.npt) * kPaKeys;
+    k.lo = k.prefix ? it.klo_p : it.klo_o;
+    k.hi = k.prefix ? p.a.prefix_len : it.khi_o;
+    return k;
 }
 
 __device__ __forceinline__ bool pa_wait(uint64_t* bar, uint32_t parity, PaCtl* ctl, int* err, int code) {
@@ -265,6 +270,16 @@ __device__ __forceinline__ bool pa_wait(uint64_t* bar, uint32_t parity, PaCtl* c
 }
 __device__ __forceinline__ bool pa_wait_warp(uint64_t* bar, uint32_t parity, PaCtl* ctl, int* err, int code) {
     return __all_sync(0xffffffffu, pa_wait(bar, parity, ctl, err, code));
+}
+
+// The CTA's k-th item, or -1 after the last (or when a wait ran out).  Eleven warps take each item; with the last
+// of them the scheduler warp may hand out the next one.
+__device__ __forceinline__ int pa_next(PaCtl* ctl, int k, int lane, int* err) {
+    if (!pa_wait_warp(&ctl->ifull, k & 1, ctl, err, DEV_ERR_FULL_WAIT)) return -1;
+    const int i = *(volatile int*)&ctl->item;
+    __syncwarp();
+    if (lane == 0) mbar_arrive(&ctl->iempty);
+    return i;
 }
 
 __device__ __forceinline__ void tma_3d(uint32_t dst, const CUtensorMap* m, int x, int y, int z, uint64_t* bar) {
@@ -284,28 +299,33 @@ __device__ __forceinline__ void tma_4d(uint32_t dst, const CUtensorMap* m, int x
 // and stride byte offsets in 16-byte units, bit 46 the descriptor version of sm_100, bits 61-63 the swizzle.
 // K-major (Q, K): stride = 1024 between groups of 8 rows.  MN-major (V, read by columns): leading = the distance
 // between blocks of 64 columns, stride = 1024 between groups of 8 keys.
-__device__ __forceinline__ uint64_t sw128_desc(uint32_t addr, uint32_t lbo, uint32_t sbo) {
-    return (uint64_t)((addr >> 4) & 0x3FFFu) | ((uint64_t)((lbo >> 4) & 0x3FFFu) << 16) |
-           ((uint64_t)((sbo >> 4) & 0x3FFFu) << 32) | (1ull << 46) | (2ull << 61);
-}
+// The high word is the same for both; the low word is the start address and the leading offset, so that a step along K
+// is one 32-bit add.
+constexpr uint32_t kDescHi = (1024u >> 4) | (1u << 14) | (2u << 29);
+__device__ __forceinline__ uint32_t sw128_lo(uint32_t addr, uint32_t lbo) { return (addr >> 4) | ((lbo >> 4) << 16); }
 // Instruction descriptor of kind::f16: D fp32, A and B fp16 or bf16, B MN-major if trans_b, M = 128.
 __host__ __device__ constexpr uint32_t idesc_f16(bool bf16, int n, bool trans_b) {
     return (1u << 4) | ((bf16 ? 1u : 0u) << 7) | ((bf16 ? 1u : 0u) << 10) | ((trans_b ? 1u : 0u) << 16) |
            ((uint32_t)(n >> 3) << 17) | ((uint32_t)(128 >> 4) << 24);
 }
-__device__ __forceinline__ void mma_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t acc) {
+__device__ __forceinline__ void mma_ss(uint32_t d, uint32_t a, uint32_t b, uint32_t idesc, uint32_t acc) {
     asm volatile(
-        "{\n .reg .pred p;\n setp.ne.b32 p, %4, 0;\n"
-        " tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n}\n" ::"r"(d),
-        "l"(a), "l"(b), "r"(idesc), "r"(acc)
+        "{\n .reg .pred p;\n .reg .b64 da, db;\n setp.ne.b32 p, %4, 0;\n mov.b64 da, {%1, %5};\n mov.b64 db, {%2, %5};\n"
+        " tcgen05.mma.cta_group::1.kind::f16 [%0], da, db, %3, p;\n}\n" ::"r"(d),
+        "r"(a), "r"(b), "r"(idesc), "r"(acc), "n"(kDescHi)
         : "memory");
 }
-__device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, uint32_t acc) {
+__device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint32_t b, uint32_t idesc, uint32_t acc) {
     asm volatile(
-        "{\n .reg .pred p;\n setp.ne.b32 p, %4, 0;\n"
-        " tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n}\n" ::"r"(d),
-        "r"(a), "l"(b), "r"(idesc), "r"(acc)
+        "{\n .reg .pred p;\n .reg .b64 db;\n setp.ne.b32 p, %4, 0;\n mov.b64 db, {%2, %5};\n"
+        " tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], db, %3, p;\n}\n" ::"r"(d),
+        "r"(a), "r"(b), "r"(idesc), "r"(acc), "n"(kDescHi)
         : "memory");
+}
+__device__ __forceinline__ bool elect_one() {
+    uint32_t e;
+    asm volatile("{\n .reg .pred p;\n elect.sync _|p, 0xffffffff;\n selp.u32 %0, 1, 0, p;\n}\n" : "=r"(e));
+    return e != 0;
 }
 __device__ __forceinline__ void pa_commit(uint64_t* bar) {
     asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(smem_u32(bar))
@@ -403,6 +423,9 @@ __global__ void __launch_bounds__(kPaThreads, 1) k_pattn(const __grid_constant__
         mbar_init(&ctl->mready, 128);
         mbar_init(&ctl->mdone, 128);
         mbar_init(&ctl->done, 1);
+        mbar_init(&ctl->ifull, 1);
+        mbar_init(&ctl->iempty, 11);
+        mbar_init(&ctl->claim, 1);
         ctl->abort = 0;
         fence_mbar_init();
     }
@@ -449,6 +472,9 @@ __global__ void __launch_bounds__(kPaThreads, 1) k_pattn(const __grid_constant__
     const int n_items = (p.cp * p.n_pt + ustart[a.n_req]) * a.pool.n_kv_heads;
     const int ps = a.pool.page_size, G = p.G;
 
+    // the softmax warps keep a row of 128 scores in registers: 8 x 32 x 216 + 4 x 32 x 72 = 384 x 168
+    if (warp >= 8) {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 72;");
     if (warp == 8) {
         // ---------------- TMA ----------------
         uint32_t pos = 0;
@@ -456,8 +482,10 @@ __global__ void __launch_bounds__(kPaThreads, 1) k_pattn(const __grid_constant__
         const int box = min(ps, kPaKeys), npg = kPaKeys / box;  // pages per key tile
         const uint32_t page_bytes = (uint32_t)box * 128u * NH;
         bool ok = true;
-        for (int i = blockIdx.x; i < n_items && ok; i += gridDim.x) {
+        for (int k = 0; ok; ++k) {
             PaItem it;
+            const int i = pa_next(ctl, k, lane, p.err);
+            if (i < 0) break;
             if (!pa_item(p, ustart, i, it) || it.n == 0) continue;
             if (nq > 0 && !pa_wait_warp(&ctl->qempty, (nq - 1) & 1, ctl, p.err, DEV_ERR_EMPTY_WAIT)) break;
             if (lane == 0) {
@@ -469,7 +497,7 @@ __global__ void __launch_bounds__(kPaThreads, 1) k_pattn(const __grid_constant__
             }
             ++nq;
             for (int t = 0; t < it.n; ++t) {
-                const PaTile kt = pa_tile(p, it, it.v0 + t);
+                const PaTile kt = pa_tile(p, it, t);
                 // lane g < npg: page g of the tile
                 const int key = kt.k0 + lane * box;
                 const bool want = lane < npg && key < kt.hi && key + box > kt.lo;
@@ -506,124 +534,134 @@ __global__ void __launch_bounds__(kPaThreads, 1) k_pattn(const __grid_constant__
         for (uint32_t q = pos > NST ? pos - NST : 0; q < pos; ++q) mbar_wait(&ctl->full[q % NST], (q / NST) & 1);
         if (nq > 0) mbar_wait(&ctl->qfull, (nq - 1) & 1);
     } else if (warp == 9) {
-        // ---------------- MMA issue ----------------
-        if (lane == 0) {
-            constexpr uint32_t id_s = idesc_f16(BF, kPaKeys, false), id_o = idesc_f16(BF, HD, true);
-            uint32_t pos = 0, fixes = 0, np[2] = {0, 0};
-            int nq = 0;
-            bool ok = true;
-            auto wait_k = [&](uint32_t q) {
-                ok = ok && pa_wait(&ctl->full[q % NST], (q / NST) & 1, ctl, p.err, DEV_ERR_FULL_WAIT);
-                pa_fence_after();
-            };
-            auto score = [&](int slot, int qt, uint32_t q) {
-                const uint32_t qa = qs + qt * TILE, ka = kvs + (q % NST) * TILE;
+        // ---------------- MMA issue: the warp walks together, one elected lane issues ----------------
+        constexpr uint32_t id_s = idesc_f16(BF, kPaKeys, false), id_o = idesc_f16(BF, HD, true);
+        const bool leader = elect_one();
+        uint32_t pos = 0, fixes = 0, np[2] = {0, 0};
+        int nq = 0;
+        bool ok = true;
+        auto wait_k = [&](uint32_t q) {
+            ok = ok && pa_wait_warp(&ctl->full[q % NST], (q / NST) & 1, ctl, p.err, DEV_ERR_FULL_WAIT);
+        };
+        auto commit = [&](uint64_t* bar) {
+            if (leader) pa_commit(bar);
+        };
+        auto score = [&](int slot, int qt, uint32_t q) {
+            pa_fence_after();
+            const uint32_t qa = sw128_lo(qs + qt * TILE, 16), ka = sw128_lo(kvs + (q % NST) * TILE, 16), d = tmem + slot * 128;
+            if (leader) {
 #pragma unroll
-                for (int ks = 0; ks < HD / 16; ++ks)
-                    mma_ss(tmem + slot * 128, sw128_desc(qa + (ks >> 2) * kPaHalf + (ks & 3) * 32, 16, 1024),
-                           sw128_desc(ka + (ks >> 2) * kPaHalf + (ks & 3) * 32, 16, 1024), id_s, ks > 0);
-                pa_commit(&ctl->sfull[slot]);
-            };
-            auto wait_p = [&](int slot) {
-                ok = ok && pa_wait(&ctl->pready[slot], np[slot] & 1, ctl, p.err, DEV_ERR_FULL_WAIT);
-                ++np[slot];
-                pa_fence_after();
-            };
-            auto wait_v = [&](const PaItem& it, int t, uint32_t q) {
-                wait_k(q);
-                if (!ok) return;
-                const PaTile kt = pa_tile(p, it, it.v0 + t);
-                const int st = q % NST;
-                if (kt.k0 < kt.lo || kt.k0 + kPaKeys > kt.hi || ctl->okmask[(q >> 1) & 15] != 0xFFu) {
-                    ok = pa_wait(&ctl->fixed[st], fixes >> st & 1, ctl, p.err, DEV_ERR_FULL_WAIT);
-                    fixes ^= 1u << st;
+                for (int ks = 0; ks < HD / 16; ++ks) {
+                    const uint32_t o = ((ks >> 2) * kPaHalf + (ks & 3) * 32) >> 4;
+                    mma_ss(d, qa + o, ka + o, id_s, ks > 0);
                 }
-            };
-            auto value = [&](int slot, bool acc, uint32_t q) {
-                const uint32_t va = kvs + (q % NST) * TILE;
+                pa_commit(&ctl->sfull[slot]);
+            }
+        };
+        auto wait_p = [&](int slot) {
+            ok = ok && pa_wait_warp(&ctl->pready[slot], np[slot] & 1, ctl, p.err, DEV_ERR_FULL_WAIT);
+            ++np[slot];
+        };
+        auto wait_v = [&](const PaItem& it, int t, uint32_t q) {
+            wait_k(q);
+            if (!ok) return;
+            const PaTile kt = pa_tile(p, it, t);
+            const int st = q % NST;
+            if (kt.k0 < kt.lo || kt.k0 + kPaKeys > kt.hi || ctl->okmask[(q >> 1) & 15] != 0xFFu) {
+                ok = pa_wait_warp(&ctl->fixed[st], fixes >> st & 1, ctl, p.err, DEV_ERR_FULL_WAIT);
+                fixes ^= 1u << st;
+            }
+        };
+        auto value = [&](int slot, bool acc, uint32_t q) {
+            pa_fence_after();
+            const uint32_t va = sw128_lo(kvs + (q % NST) * TILE, kPaHalf), d = tmem + 256 + slot * HD, pa = tmem + slot * 128;
+            if (leader) {
 #pragma unroll
-                for (int ks = 0; ks < kPaKeys / 16; ++ks)
-                    mma_ts(tmem + 256 + slot * HD, tmem + slot * 128 + ks * 8, sw128_desc(va + ks * 2048, kPaHalf, 1024), id_o,
-                           acc || ks > 0);
+                for (int ks = 0; ks < kPaKeys / 16; ++ks) mma_ts(d, pa + ks * 8, va + ks * (2048 >> 4), id_o, acc || ks > 0);
                 pa_commit(&ctl->ofull[slot]);
-            };
-            for (int i = blockIdx.x; i < n_items && ok; i += gridDim.x) {
-                PaItem it;
-                if (!pa_item(p, ustart, i, it) || it.n == 0) continue;
-                ok = pa_wait(&ctl->qfull, nq & 1, ctl, p.err, DEV_ERR_FULL_WAIT);
-                ++nq;
-                const uint32_t k0 = pos;
-                const int n = it.n;
-                pos += 2 * n;
-                wait_k(k0);
-                if (!ok) break;
-                if (it.pair) {
-                    score(0, 0, k0);
-                    score(1, 1, k0);
-                    pa_commit(&ctl->empty[k0 % NST]);
-                    if (n == 1) pa_commit(&ctl->qempty);
-                    for (int t = 0; t < n && ok; ++t) {
-                        const uint32_t v = k0 + 2 * t + 1, kn = v + 1;
-                        wait_v(it, t, v);
-                        if (ok) wait_p(0);
+            }
+        };
+        for (int k = 0;; ++k) {
+            PaItem it;
+            const int i = pa_next(ctl, k, lane, p.err);
+            if (i < 0) break;
+            if (!pa_item(p, ustart, i, it) || it.n == 0) continue;
+            ok = pa_wait_warp(&ctl->qfull, nq & 1, ctl, p.err, DEV_ERR_FULL_WAIT);
+            ++nq;
+            const uint32_t k0 = pos;
+            const int n = it.n;
+            pos += 2 * n;
+            wait_k(k0);
+            if (!ok) break;
+            if (it.pair) {
+                score(0, 0, k0);
+                score(1, 1, k0);
+                commit(&ctl->empty[k0 % NST]);
+                if (n == 1) commit(&ctl->qempty);
+                for (int t = 0; t < n && ok; ++t) {
+                    const uint32_t v = k0 + 2 * t + 1, kn = v + 1;
+                    wait_v(it, t, v);
+                    if (ok) wait_p(0);
+                    if (!ok) break;
+                    value(0, t > 0, v);
+                    if (t + 1 < n) {
+                        wait_k(kn);
                         if (!ok) break;
-                        value(0, t > 0, v);
-                        if (t + 1 < n) {
-                            wait_k(kn);
-                            if (!ok) break;
-                            score(0, 0, kn);
-                        }
-                        wait_p(1);
-                        if (!ok) break;
-                        value(1, t > 0, v);
-                        pa_commit(&ctl->empty[v % NST]);
-                        if (t + 1 < n) {
-                            score(1, 1, kn);
-                            pa_commit(&ctl->empty[kn % NST]);
-                            if (t + 2 == n) pa_commit(&ctl->qempty);
-                        }
+                        score(0, 0, kn);
                     }
-                } else {
-                    score(0, 0, k0);
-                    pa_commit(&ctl->empty[k0 % NST]);
-                    if (n > 1) {
-                        wait_k(k0 + 2);
-                        if (!ok) break;
-                        score(1, 0, k0 + 2);
-                        pa_commit(&ctl->empty[(k0 + 2) % NST]);
+                    wait_p(1);
+                    if (!ok) break;
+                    value(1, t > 0, v);
+                    commit(&ctl->empty[v % NST]);
+                    if (t + 1 < n) {
+                        score(1, 1, kn);
+                        commit(&ctl->empty[kn % NST]);
+                        if (t + 2 == n) commit(&ctl->qempty);
                     }
-                    if (n <= 2) pa_commit(&ctl->qempty);
-                    for (int t = 0; t < n && ok; ++t) {
-                        const uint32_t v = k0 + 2 * t + 1, kn = v + 3;
-                        wait_v(it, t, v);
-                        if (ok) wait_p(t & 1);
+                }
+            } else {
+                score(0, 0, k0);
+                commit(&ctl->empty[k0 % NST]);
+                if (n > 1) {
+                    wait_k(k0 + 2);
+                    if (!ok) break;
+                    score(1, 0, k0 + 2);
+                    commit(&ctl->empty[(k0 + 2) % NST]);
+                }
+                if (n <= 2) commit(&ctl->qempty);
+                for (int t = 0; t < n && ok; ++t) {
+                    const uint32_t v = k0 + 2 * t + 1, kn = v + 3;
+                    wait_v(it, t, v);
+                    if (ok) wait_p(t & 1);
+                    if (!ok) break;
+                    value(t & 1, t > 1, v);
+                    commit(&ctl->empty[v % NST]);
+                    if (t + 2 < n) {
+                        wait_k(kn);
                         if (!ok) break;
-                        value(t & 1, t > 1, v);
-                        pa_commit(&ctl->empty[v % NST]);
-                        if (t + 2 < n) {
-                            wait_k(kn);
-                            if (!ok) break;
-                            score(t & 1, 0, kn);
-                            pa_commit(&ctl->empty[kn % NST]);
-                            if (t + 3 == n) pa_commit(&ctl->qempty);
-                        }
+                        score(t & 1, 0, kn);
+                        commit(&ctl->empty[kn % NST]);
+                        if (t + 3 == n) commit(&ctl->qempty);
                     }
                 }
             }
-            // every MMA issued above has completed before the tensor memory is released
-            pa_commit(&ctl->done);
-            if (!mbar_wait(&ctl->done, 0)) set_dev_error(p.err, DEV_ERR_FULL_WAIT);
+            if (!ok) break;
         }
+        // every MMA issued above has completed before the tensor memory is released
+        commit(&ctl->done);
+        if (!mbar_wait(&ctl->done, 0)) set_dev_error(p.err, DEV_ERR_FULL_WAIT);
         __syncwarp();
     } else if (warp == 10) {
         // ---------------- V rows that no row of the item may see become zero ----------------
         uint32_t pos = 0;
         bool ok = true;
-        for (int i = blockIdx.x; i < n_items && ok; i += gridDim.x) {
+        for (int k = 0; ok; ++k) {
             PaItem it;
+            const int i = pa_next(ctl, k, lane, p.err);
+            if (i < 0) break;
             if (!pa_item(p, ustart, i, it) || it.n == 0) continue;
             for (int t = 0; t < it.n && ok; ++t) {
-                const PaTile kt = pa_tile(p, it, it.v0 + t);
+                const PaTile kt = pa_tile(p, it, t);
 #pragma unroll
                 for (int kv = 0; kv < 2; ++kv) {
                     const int st = pos % NST;
@@ -650,7 +688,46 @@ __global__ void __launch_bounds__(kPaThreads, 1) k_pattn(const __grid_constant__
                 }
             }
         }
-    } else if (warp < 8) {
+    } else {
+        // ---------------- scheduler ----------------
+        // The grid has one CTA per item; a running CTA takes over CTAs that have not started (cluster launch
+        // control), so unequal items even out over the SMs and set-up is paid once per SM.
+        if (lane == 0) {
+            int i = blockIdx.x < n_items ? (int)blockIdx.x : -1, claims = 0;
+            for (int k = 0;; ++k) {
+                if (k > 0 && !pa_wait(&ctl->iempty, (k - 1) & 1, ctl, p.err, DEV_ERR_EMPTY_WAIT)) break;
+                *(volatile int*)&ctl->item = i;
+                mbar_arrive(&ctl->ifull);
+                if (i < 0) break;
+                do {
+                    mbar_arrive_expect_tx(&ctl->claim, 16);
+                    asm volatile("clusterlaunchcontrol.try_cancel.async.shared::cta.mbarrier::complete_tx::bytes.b128 [%0], [%1];" ::"r"(
+                                     smem_u32(&ctl->claimed)),
+                                 "r"(smem_u32(&ctl->claim))
+                                 : "memory");
+                    if (!mbar_wait(&ctl->claim, claims & 1)) {
+                        set_dev_error(p.err, DEV_ERR_FULL_WAIT);
+                        *(volatile int*)&ctl->abort = 1;
+                    }
+                    ++claims;
+                    uint32_t got, x;
+                    asm volatile(
+                        "{\n .reg .pred p;\n .reg .b128 r;\n ld.shared.b128 r, [%2];\n"
+                        " clusterlaunchcontrol.query_cancel.is_canceled.pred.b128 p, r;\n selp.u32 %0, 1, 0, p;\n"
+                        " mov.u32 %1, 0;\n @p clusterlaunchcontrol.query_cancel.get_first_ctaid::x.b32.b128 %1, r;\n}\n"
+                        : "=r"(got), "=r"(x)
+                        : "r"(smem_u32(&ctl->claimed))
+                        : "memory");
+                    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+                    i = got ? (int)x : -1;
+                } while (i >= n_items && !*(volatile int*)&ctl->abort);
+                if (*(volatile int*)&ctl->abort) i = -1;
+            }
+        }
+        __syncwarp();
+    }
+    } else {
+        asm volatile("setmaxnreg.inc.sync.aligned.u32 216;");
         // ---------------- softmax: thread = row of its slot ----------------
         const int slot = warp >> 2, row = tid & 127;
         const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;
@@ -662,8 +739,10 @@ __global__ void __launch_bounds__(kPaThreads, 1) k_pattn(const __grid_constant__
         const float cap2 = a.softcap * kLog2e, xs = a.softcap > 0.f ? 2.f * kLog2e * a.scale / a.softcap : 0.f;
         uint32_t ns = 0, no = 0, nm = 0, tiles = 0;
         bool ok = true;
-        for (int i = blockIdx.x; i < n_items && ok; i += gridDim.x) {
+        for (int k = 0; ok; ++k) {
             PaItem it;
+            const int i = pa_next(ctl, k, lane, p.err);
+            if (i < 0) break;
             if (!pa_item(p, ustart, i, it)) continue;
             const int tok = it.tok0 + (it.pair ? slot * p.TPT : 0) + row_tok;
             const int head = it.kvh * G + row_head;
@@ -686,15 +765,23 @@ __global__ void __launch_bounds__(kPaThreads, 1) k_pattn(const __grid_constant__
             const int lo_o = W > 0 ? max(0, own + 1 - W) : 0, hi_o = seeing ? own + 1 : 0;
             const int lo_p = W > 0 ? max(0, P + own + 1 - W) : 0, hi_p = seeing ? P : 0;
             const float slope = MOD && a.alibi && live ? a.alibi[head] * kLog2e : 0.f;
+            // a warp without a row of the item lets its rows' products run on whatever S holds: nothing reads them
+            const bool idle = !__any_sync(0xffffffffu, live);
             float m = -INFINITY, l = 0.f;
             const int step = it.pair ? 1 : 2;
             bool first = true;
             for (int t = it.pair ? 0 : slot; t < it.n; t += step) {
-                const PaTile kt = pa_tile(p, it, it.v0 + t);
+                const PaTile kt = pa_tile(p, it, t);
                 const int lo = (kt.prefix ? lo_p : lo_o) - kt.k0, hi = (kt.prefix ? hi_p : hi_o) - kt.k0;
                 ok = pa_wait_warp(&ctl->sfull[slot], ns & 1, ctl, p.err, DEV_ERR_FULL_WAIT);
                 ++ns;
                 if (!ok) break;
+                if (idle) {
+                    mbar_arrive(&ctl->pready[slot]);
+                    ++no;
+                    first = false;
+                    continue;
+                }
                 pa_fence_after();
                 uint32_t y[4][32];
 #pragma unroll
@@ -702,20 +789,27 @@ __global__ void __launch_bounds__(kPaThreads, 1) k_pattn(const __grid_constant__
 #pragma unroll
                 for (int c = 0; c < 4; ++c) pa_wait_ld(y[c]);
                 if (MOD) {
-                    const float bias = kt.prefix ? slope * (float)(P + own - kt.k0) : slope * (float)(own - kt.k0);
+                    if (a.softcap > 0.f) {
 #pragma unroll
-                    for (int c = 0; c < 4; ++c)
+                        for (int c = 0; c < 4; ++c)
 #pragma unroll
-                        for (int e = 0; e < 32; ++e) {
-                            float s = __uint_as_float(y[c][e]);
-                            if (a.softcap > 0.f) {
-                                s = fmaf(__fdividef(-2.f, 1.f + ex2(s * xs)), cap2, cap2);
-                            } else {
-                                s *= sc2;
-                            }
-                            s += fmaf(slope, (float)(c * 32 + e), -bias);
-                            y[c][e] = __float_as_uint(s);
-                        }
+                            for (int e = 0; e < 32; ++e)
+                                y[c][e] = __float_as_uint(
+                                    fmaf(__fdividef(-2.f, 1.f + ex2(__uint_as_float(y[c][e]) * xs)), cap2, cap2));
+                    } else {
+#pragma unroll
+                        for (int c = 0; c < 4; ++c)
+#pragma unroll
+                            for (int e = 0; e < 32; ++e) y[c][e] = __float_as_uint(__uint_as_float(y[c][e]) * sc2);
+                    }
+                    if (a.alibi) {
+                        const float bias = slope * (float)((kt.prefix ? P : 0) + own - kt.k0);
+#pragma unroll
+                        for (int c = 0; c < 4; ++c)
+#pragma unroll
+                            for (int e = 0; e < 32; ++e)
+                                y[c][e] = __float_as_uint(__uint_as_float(y[c][e]) + fmaf(slope, (float)(c * 32 + e), -bias));
+                    }
                 }
                 const uint32_t mask = *(volatile uint32_t*)&ctl->okmask[(tiles + t) & 15];
                 if (!__all_sync(0xffffffffu, lo <= 0 && hi >= kPaKeys && mask == 0xFFu)) {
@@ -805,7 +899,7 @@ __global__ void __launch_bounds__(kPaThreads, 1) k_pattn(const __grid_constant__
                     l = l * f0 + other.y * f1;
                 }
             }
-            if (it.pair || slot == 0) {
+            if ((it.pair || slot == 0) && !idle) {
                 const size_t orow = (size_t)tok * a.n_heads + head;
                 const size_t prow = (size_t)it.split * a.n_tokens * a.n_heads + orow;
                 const float inv = l > 0.f ? 1.f / l : (l == 0.f ? 0.f : l);  // NaN stays NaN
@@ -1028,7 +1122,7 @@ int run_tc(const sd_attn_args& a, int dev, cudaStream_t st) {
     const long long items = (long long)k.n_kv_heads * ((long long)p.cp * p.n_pt + ((long long)a.n_req + a.n_tokens / pair) *
                                                        std::max(1, (own + p.ct_own - 1) / p.ct_own));
     if (items > INT32_MAX) return fail(SD_ERR_INVALID, "sd_attention_dev: too many work items");
-    const int grid = (int)std::min<long long>(items, device_sm_count(dev));
+    const int grid = (int)items;
     const bool mod = a.softcap > 0.f || a.alibi || !(a.scale > 0.f);
     if (bf) {
         if (k.head_dim == 128) return mod ? launch_tc<__nv_bfloat16, 128, true>(p, grid, st) : launch_tc<__nv_bfloat16, 128, false>(p, grid, st);
