@@ -139,7 +139,7 @@ struct PaArgs {
 struct PaCtl {
     uint64_t qfull, qempty;
     uint64_t full[8], empty[8], fixed[8];
-    uint64_t sfull[2], pready[2], ofull[2];
+    uint64_t sfull[2], pready[2][2], ofull[2];  // pready: P of the tile's first and second 64 keys
     uint64_t mready, mdone, done;
     uint64_t ifull, iempty, claim;  // hand-over of the next item; answer to the claim of another CTA's
     uint4 claimed;
@@ -370,6 +370,11 @@ __device__ __forceinline__ float ex2(float x) {
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
     return y;
 }
+__device__ __forceinline__ float rcp(float x) {
+    float y;
+    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
 template <class T> __device__ __forceinline__ uint32_t pa_pack(float lo, float hi);
 template <> __device__ __forceinline__ uint32_t pa_pack<__half>(float lo, float hi) {
     const __half2 h = __floats2half2_rn(lo, hi);
@@ -417,7 +422,8 @@ __global__ void __launch_bounds__(kPaThreads, 1) k_pattn(const __grid_constant__
         }
         for (int i = 0; i < 2; ++i) {
             mbar_init(&ctl->sfull[i], 1);
-            mbar_init(&ctl->pready[i], 128);
+            mbar_init(&ctl->pready[i][0], 128);
+            mbar_init(&ctl->pready[i][1], 128);
             mbar_init(&ctl->ofull[i], 1);
         }
         mbar_init(&ctl->mready, 128);
@@ -558,10 +564,6 @@ __global__ void __launch_bounds__(kPaThreads, 1) k_pattn(const __grid_constant__
                 pa_commit(&ctl->sfull[slot]);
             }
         };
-        auto wait_p = [&](int slot) {
-            ok = ok && pa_wait_warp(&ctl->pready[slot], np[slot] & 1, ctl, p.err, DEV_ERR_FULL_WAIT);
-            ++np[slot];
-        };
         auto wait_v = [&](const PaItem& it, int t, uint32_t q) {
             wait_k(q);
             if (!ok) return;
@@ -572,14 +574,21 @@ __global__ void __launch_bounds__(kPaThreads, 1) k_pattn(const __grid_constant__
                 fixes ^= 1u << st;
             }
         };
+        // O += P V, the first half of the keys while the softmax still computes the second
         auto value = [&](int slot, bool acc, uint32_t q) {
-            pa_fence_after();
             const uint32_t va = sw128_lo(kvs + (q % NST) * TILE, kPaHalf), d = tmem + 256 + slot * HD, pa = tmem + slot * 128;
-            if (leader) {
 #pragma unroll
-                for (int ks = 0; ks < kPaKeys / 16; ++ks) mma_ts(d, pa + ks * 8, va + ks * (2048 >> 4), id_o, acc || ks > 0);
-                pa_commit(&ctl->ofull[slot]);
+            for (int h = 0; h < 2; ++h) {
+                ok = ok && pa_wait_warp(&ctl->pready[slot][h], np[slot] & 1, ctl, p.err, DEV_ERR_FULL_WAIT);
+                if (!ok) return;
+                pa_fence_after();
+                if (leader) {
+#pragma unroll
+                    for (int ks = 4 * h; ks < 4 * h + 4; ++ks) mma_ts(d, pa + ks * 8, va + ks * (2048 >> 4), id_o, acc || ks > 0);
+                    if (h == 1) pa_commit(&ctl->ofull[slot]);
+                }
             }
+            ++np[slot];
         };
         for (int k = 0;; ++k) {
             PaItem it;
@@ -601,17 +610,15 @@ __global__ void __launch_bounds__(kPaThreads, 1) k_pattn(const __grid_constant__
                 for (int t = 0; t < n && ok; ++t) {
                     const uint32_t v = k0 + 2 * t + 1, kn = v + 1;
                     wait_v(it, t, v);
-                    if (ok) wait_p(0);
-                    if (!ok) break;
                     value(0, t > 0, v);
+                    if (!ok) break;
                     if (t + 1 < n) {
                         wait_k(kn);
                         if (!ok) break;
                         score(0, 0, kn);
                     }
-                    wait_p(1);
-                    if (!ok) break;
                     value(1, t > 0, v);
+                    if (!ok) break;
                     commit(&ctl->empty[v % NST]);
                     if (t + 1 < n) {
                         score(1, 1, kn);
@@ -632,9 +639,8 @@ __global__ void __launch_bounds__(kPaThreads, 1) k_pattn(const __grid_constant__
                 for (int t = 0; t < n && ok; ++t) {
                     const uint32_t v = k0 + 2 * t + 1, kn = v + 3;
                     wait_v(it, t, v);
-                    if (ok) wait_p(t & 1);
-                    if (!ok) break;
                     value(t & 1, t > 1, v);
+                    if (!ok) break;
                     commit(&ctl->empty[v % NST]);
                     if (t + 2 < n) {
                         wait_k(kn);
@@ -761,9 +767,10 @@ __global__ void __launch_bounds__(kPaThreads, 1) k_pattn(const __grid_constant__
                 }
             }
             const int P = a.prefix_len, W = a.window;
-            const bool seeing = live && own >= 0;
-            const int lo_o = W > 0 ? max(0, own + 1 - W) : 0, hi_o = seeing ? own + 1 : 0;
-            const int lo_p = W > 0 ? max(0, P + own + 1 - W) : 0, hi_p = seeing ? P : 0;
+            // lanes without a row see everything, so that they call for no masking; nothing reads what they compute
+            const bool seeing = own >= 0;
+            const int lo_o = W > 0 && live ? max(0, own + 1 - W) : 0, hi_o = !live ? INT32_MAX : seeing ? own + 1 : 0;
+            const int lo_p = W > 0 && live ? max(0, P + own + 1 - W) : 0, hi_p = !live ? INT32_MAX : seeing ? P : 0;
             const float slope = MOD && a.alibi && live ? a.alibi[head] * kLog2e : 0.f;
             // a warp without a row of the item lets its rows' products run on whatever S holds: nothing reads them
             const bool idle = !__any_sync(0xffffffffu, live);
@@ -777,7 +784,8 @@ __global__ void __launch_bounds__(kPaThreads, 1) k_pattn(const __grid_constant__
                 ++ns;
                 if (!ok) break;
                 if (idle) {
-                    mbar_arrive(&ctl->pready[slot]);
+                    mbar_arrive(&ctl->pready[slot][0]);
+                    mbar_arrive(&ctl->pready[slot][1]);
                     ++no;
                     first = false;
                     continue;
@@ -795,7 +803,7 @@ __global__ void __launch_bounds__(kPaThreads, 1) k_pattn(const __grid_constant__
 #pragma unroll
                             for (int e = 0; e < 32; ++e)
                                 y[c][e] = __float_as_uint(
-                                    fmaf(__fdividef(-2.f, 1.f + ex2(__uint_as_float(y[c][e]) * xs)), cap2, cap2));
+                                    fmaf(rcp(1.f + ex2(__uint_as_float(y[c][e]) * xs)), -2.f * cap2, cap2));
                     } else {
 #pragma unroll
                         for (int c = 0; c < 4; ++c)
@@ -814,18 +822,23 @@ __global__ void __launch_bounds__(kPaThreads, 1) k_pattn(const __grid_constant__
                 const uint32_t mask = *(volatile uint32_t*)&ctl->okmask[(tiles + t) & 15];
                 if (!__all_sync(0xffffffffu, lo <= 0 && hi >= kPaKeys && mask == 0xFFu)) {
 #pragma unroll
-                    for (int c = 0; c < 4; ++c)
+                    for (int c = 0; c < 4; ++c) {
+                        // keys of this quarter: bits [lo, hi) of those that were loaded
+                        const int l0 = min(max(lo - c * 32, 0), 32), h0 = min(max(hi - c * 32, 0), 32);
+                        uint32_t vis = (h0 < 32 ? (1u << h0) - 1u : 0xffffffffu) & ~(l0 < 32 ? (1u << l0) - 1u : 0xffffffffu);
+                        if (!(mask >> (2 * c) & 1)) vis &= 0xffff0000u;
+                        if (!(mask >> (2 * c + 1) & 1)) vis &= 0x0000ffffu;
 #pragma unroll
-                        for (int e = 0; e < 32; ++e) {
-                            const int k = c * 32 + e;
-                            if (!(k >= lo && k < hi && (mask >> (k >> 4) & 1))) y[c][e] = 0xff800000u;  // -infinity
-                        }
+                        for (int e = 0; e < 32; ++e)
+                            if (!(vis & (1u << e))) y[c][e] = 0xff800000u;  // -infinity
+                    }
                 }
                 float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
                 for (int c = 0; c < 4; ++c)
 #pragma unroll
-                    for (int e = 0; e < 32; ++e) mx[e & 3] = fmaxf(mx[e & 3], __uint_as_float(y[c][e]));
+                    for (int e = 0; e < 32; e += 2)
+                        mx[(e >> 1) & 3] = fmaxf(mx[(e >> 1) & 3], fmaxf(__uint_as_float(y[c][e]), __uint_as_float(y[c][e + 1])));
                 float top = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3]));
                 if (!MOD) top *= sc2;
                 float factor = 1.f;
@@ -850,25 +863,26 @@ __global__ void __launch_bounds__(kPaThreads, 1) k_pattn(const __grid_constant__
                     }
                 }
                 const float ref = (m == -INFINITY ? 0.f : m) - kShift;
-                float sum[4] = {0.f, 0.f, 0.f, 0.f};
+                const float2 ref2 = make_float2(-ref, -ref), one2 = make_float2(MOD ? 1.f : sc2, MOD ? 1.f : sc2);
+                float2 sum[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
 #pragma unroll
                 for (int h = 0; h < 2; ++h) {
                     uint32_t pk[32];
 #pragma unroll
                     for (int e = 0; e < 32; ++e) {
                         const int c = h * 2 + (e >> 4), x = (e & 15) * 2;
-                        const float s0 = __uint_as_float(y[c][x]), s1 = __uint_as_float(y[c][x + 1]);
-                        const float p0 = ex2(MOD ? s0 - ref : fmaf(s0, sc2, -ref)), p1 = ex2(MOD ? s1 - ref : fmaf(s1, sc2, -ref));
-                        sum[(e & 1) * 2] += p0;
-                        sum[(e & 1) * 2 + 1] += p1;
-                        pk[e] = pa_pack<T>(p0, p1);
+                        float2 z = __ffma2_rn(make_float2(__uint_as_float(y[c][x]), __uint_as_float(y[c][x + 1])), one2, ref2);
+                        z.x = ex2(z.x);
+                        z.y = ex2(z.y);
+                        sum[e & 1] = __fadd2_rn(sum[e & 1], z);
+                        pk[e] = pa_pack<T>(z.x, z.y);
                     }
                     pa_st32(ts + h * 32, pk);
+                    pa_wait_st();
+                    pa_fence_before();
+                    mbar_arrive(&ctl->pready[slot][h]);
                 }
-                l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
-                pa_wait_st();
-                pa_fence_before();
-                mbar_arrive(&ctl->pready[slot]);
+                l += (sum[0].x + sum[0].y) + (sum[1].x + sum[1].y);
                 ++no;
                 first = false;
             }
