@@ -17,6 +17,9 @@
 
 using namespace sd;
 
+#ifndef PA_POLY
+#define PA_POLY 0
+#endif
 namespace sd {
 namespace {
 
@@ -138,13 +141,21 @@ struct PaArgs {
 
 struct PaCtl {
     uint64_t qfull, qempty;
-    uint64_t full[8], empty[8], fixed[8];
-    uint64_t sfull[2], pready[2][2], ofull[2];  // pready: P of the tile's first and second 64 keys
+    uint64_t full[16], empty[16], fixed[16];
+    uint64_t sfull[2][2], pready[2][2];  // [slot][half of the tile's keys]: S and P written
+    // A parity wait tells a phase from its neighbour only: ofull (one phase per half's product) is waited for where the
+    // last but one product is known to be complete, odone has one phase per item.
+    uint64_t ofull[2], odone[2];
     uint64_t mready, mdone, done;
     uint64_t ifull, iempty, claim;  // hand-over of the next item; answer to the claim of another CTA's
     uint4 claimed;
     int item;
-    uint32_t okmask[16];  // per key tile, in turn: which of its 16-key groups were loaded
+    // per key tile (in turn) and half: which of its 16-key groups were loaded (bits 0-3), and whether V has rows that no
+    // row of the item may see (bit 8)
+    uint32_t okmask[16][2];
+    int pages[16][8];   // per key tile: its page ids, -1 where there is none to load
+    uint64_t fq[16];    // a request for zero rows is posted
+    int4 fix[16];       // stage (-1: no more), its phase, first and last + 1 row to keep | mask << 16
     float2 ml1[128];      // slot 1's state at a merge
     uint32_t tmem;
     int abort;
@@ -261,18 +272,23 @@ __device__ __forceinline__ PaTile pa_tile(const PaArgs& p, const PaItem& it, int
     return k;
 }
 
-__device__ __forceinline__ bool pa_wait(uint64_t* bar, uint32_t parity, PaCtl* ctl, int* err, int code) {
+// Waits of one thread and of a whole warp; false once any wait of the CTA has run out.
+__device__ __noinline__ bool pa_wait_slow(uint64_t* bar, uint32_t parity, PaCtl* ctl, int* err, int code) {
     if (*(volatile int*)&ctl->abort) return false;
     if (mbar_wait(bar, parity)) return true;
     set_dev_error(err, code);
     *(volatile int*)&ctl->abort = 1;
     return false;
 }
+__device__ __forceinline__ bool pa_wait(uint64_t* bar, uint32_t parity, PaCtl* ctl, int* err, int code) {
+    return mbar_try_wait(bar, parity) || pa_wait_slow(bar, parity, ctl, err, code);
+}
 __device__ __forceinline__ bool pa_wait_warp(uint64_t* bar, uint32_t parity, PaCtl* ctl, int* err, int code) {
-    return __all_sync(0xffffffffu, pa_wait(bar, parity, ctl, err, code));
+    if (__all_sync(0xffffffffu, mbar_try_wait(bar, parity))) return true;
+    return __all_sync(0xffffffffu, pa_wait_slow(bar, parity, ctl, err, code));
 }
 
-// The CTA's k-th item, or -1 after the last (or when a wait ran out).  Eleven warps take each item; with the last
+// The CTA's k-th item, or -1 after the last (or when a wait ran out).  Ten warps take each item; with the last
 // of them the scheduler warp may hand out the next one.
 __device__ __forceinline__ int pa_next(PaCtl* ctl, int k, int lane, int* err) {
     if (!pa_wait_warp(&ctl->ifull, k & 1, ctl, err, DEV_ERR_FULL_WAIT)) return -1;
@@ -375,6 +391,33 @@ __device__ __forceinline__ float rcp(float x) {
     asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
     return y;
 }
+// 2^z of two values on the FMA pipe: z = i + f with i the nearest integer (added to 1.5 2^23 it stands in the low
+// mantissa bits), 2^f by a polynomial of degree 4 on [-1/2, 1/2] with constant term 1 (minimax, relative error
+// 2.8e-6), i added to the exponent.  Below -127 the result is 0.
+__device__ __forceinline__ float2 ex2_fma(float2 z) {
+    z.x = fmaxf(z.x, -127.f);
+    z.y = fmaxf(z.y, -127.f);
+    const float2 t = __fadd2_rn(z, make_float2(12582912.f, 12582912.f));
+    const float2 f = __fadd2_rn(z, __ffma2_rn(t, make_float2(-1.f, -1.f), make_float2(12582912.f, 12582912.f)));
+    float2 q = __ffma2_rn(f, make_float2(0.009582852944731712f, 0.009582852944731712f),
+                          make_float2(0.055906426161527634f, 0.055906426161527634f));
+    q = __ffma2_rn(f, q, make_float2(0.24024099111557007f, 0.24024099111557007f));
+    q = __ffma2_rn(f, q, make_float2(0.6931241750717163f, 0.6931241750717163f));
+    q = __ffma2_rn(f, q, make_float2(1.f, 1.f));
+    return make_float2(__uint_as_float(__float_as_uint(q.x) + (__float_as_uint(t.x) << 23)),
+                       __uint_as_float(__float_as_uint(q.y) + (__float_as_uint(t.y) << 23)));
+}
+// tanh of two values in [-1, 1]: x times a polynomial in x^2 (minimax, relative error 5.5e-8).
+__device__ __forceinline__ float2 tanh_small(float2 x) {
+    const float2 u = __fmul2_rn(x, x);
+    float2 q = make_float2(0.0010582432f, 0.0010582432f);
+    q = __ffma2_rn(u, q, make_float2(-0.0062592784f, -0.0062592784f));
+    q = __ffma2_rn(u, q, make_float2(0.020359693f, 0.020359693f));
+    q = __ffma2_rn(u, q, make_float2(-0.053498674f, -0.053498674f));
+    q = __ffma2_rn(u, q, make_float2(0.13326408f, 0.13326408f));
+    q = __ffma2_rn(u, q, make_float2(-0.33332986f, -0.33332986f));
+    return __ffma2_rn(__fmul2_rn(x, u), q, x);
+}
 template <class T> __device__ __forceinline__ uint32_t pa_pack(float lo, float hi);
 template <> __device__ __forceinline__ uint32_t pa_pack<__half>(float lo, float hi) {
     const __half2 h = __floats2half2_rn(lo, hi);
@@ -386,10 +429,10 @@ template <> __device__ __forceinline__ uint32_t pa_pack<__nv_bfloat16>(float lo,
 }
 
 template <int HD>
-constexpr int pa_stages() { return HD == 128 ? 4 : 8; }
+constexpr int pa_stages() { return HD == 128 ? 8 : 16; }
 template <int HD>
 constexpr size_t pa_smem(int n_req) {
-    return (size_t)2 * (HD / 64) * kPaHalf + (size_t)pa_stages<HD>() * (HD / 64) * kPaHalf + sizeof(PaCtl) +
+    return (size_t)2 * (HD / 64) * kPaHalf + (size_t)pa_stages<HD>() * (HD / 64) * (kPaHalf / 2) + sizeof(PaCtl) +
            ((size_t)n_req + 1) * 4 + 1024;
 }
 
@@ -398,16 +441,19 @@ template <class T, int HD, bool MOD>
 __global__ void __launch_bounds__(kPaThreads, 1) k_pattn(const __grid_constant__ PaArgs p) {
     constexpr int NST = pa_stages<HD>();
     constexpr int NH = HD / 64;                 // 64-element halves of a row
-    constexpr uint32_t TILE = NH * kPaHalf;     // bytes of a Q, K or V tile
+    constexpr uint32_t TILE = NH * kPaHalf;     // bytes of a Q tile
+    constexpr uint32_t STAGE = TILE / 2;        // bytes of a ring stage: K or V of 64 keys, [64-element half][key]
+    constexpr uint32_t kSHalf = kPaHalf / 2;
     constexpr bool BF = sizeof(T) == 2 && !std::is_same<T, __half>::value;
     // fp16 weights are kept 2^6 above the running maximum's scale (at most 2^14 with the 2^8 slack), so that small
     // ones stay in the type's normal range
     constexpr float kShift = BF ? 0.f : 6.f;
     constexpr float kSlack = 8.f;
+    constexpr int POLY = PA_POLY;
     extern __shared__ uint8_t raw[];
     uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(raw) + 1023) & ~(uintptr_t)1023);
     const uint32_t qs = smem_u32(smem), kvs = qs + 2 * TILE;
-    PaCtl* ctl = reinterpret_cast<PaCtl*>(smem + (2 + NST) * TILE);
+    PaCtl* ctl = reinterpret_cast<PaCtl*>(smem + 2 * TILE + NST * STAGE);
     int* ustart = reinterpret_cast<int*>(ctl + 1);
     const sd_attn_args& a = p.a;
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
@@ -417,20 +463,23 @@ __global__ void __launch_bounds__(kPaThreads, 1) k_pattn(const __grid_constant__
         mbar_init(&ctl->qempty, 1);
         for (int i = 0; i < NST; ++i) {
             mbar_init(&ctl->full[i], 1);
-            mbar_init(&ctl->empty[i], 2);
+            mbar_init(&ctl->empty[i], 1);
             mbar_init(&ctl->fixed[i], 1);
         }
+        for (int i = 0; i < 16; ++i) mbar_init(&ctl->fq[i], 1);
         for (int i = 0; i < 2; ++i) {
-            mbar_init(&ctl->sfull[i], 1);
-            mbar_init(&ctl->pready[i][0], 128);
-            mbar_init(&ctl->pready[i][1], 128);
+            for (int h = 0; h < 2; ++h) {
+                mbar_init(&ctl->sfull[i][h], 1);
+                mbar_init(&ctl->pready[i][h], 4);
+            }
             mbar_init(&ctl->ofull[i], 1);
+            mbar_init(&ctl->odone[i], 1);
         }
         mbar_init(&ctl->mready, 128);
         mbar_init(&ctl->mdone, 128);
         mbar_init(&ctl->done, 1);
         mbar_init(&ctl->ifull, 1);
-        mbar_init(&ctl->iempty, 11);
+        mbar_init(&ctl->iempty, 10);
         mbar_init(&ctl->claim, 1);
         ctl->abort = 0;
         fence_mbar_init();
@@ -478,21 +527,80 @@ __global__ void __launch_bounds__(kPaThreads, 1) k_pattn(const __grid_constant__
     const int n_items = (p.cp * p.n_pt + ustart[a.n_req]) * a.pool.n_kv_heads;
     const int ps = a.pool.page_size, G = p.G;
 
-    // the softmax warps keep a row of 128 scores in registers: 8 x 32 x 216 + 4 x 32 x 72 = 384 x 168
-    if (warp >= 8) {
-    asm volatile("setmaxnreg.dec.sync.aligned.u32 72;");
+
     if (warp == 8) {
         // ---------------- TMA ----------------
-        uint32_t pos = 0;
+        uint32_t pos = 0, tiles = 0, fixes = 0;
         int nq = 0;
-        const int box = min(ps, kPaKeys), npg = kPaKeys / box;  // pages per key tile
-        const uint32_t page_bytes = (uint32_t)box * 128u * NH;
+        const int lps = 31 - __clz(ps), box = min(ps, kPaKeys / 2), nb = kPaKeys / 2 / box;  // boxes per stage and 64 elements
+        const int npg = kPaKeys / min(ps, kPaKeys);                                          // pages per tile
+        const uint32_t box_bytes = (uint32_t)box * 128u;
+        // lane NH g + j brings 64-element half j of box g of a stage; lane g < npg reads the id of page g of a tile
+        const int g = lane / NH, j = lane % NH;
+        const bool issues = g < nb;
+        const uint32_t dst0 = kvs + j * kSHalf + g * box * 128;
         bool ok = true;
         for (int k = 0; ok; ++k) {
             PaItem it;
             const int i = pa_next(ctl, k, lane, p.err);
             if (i < 0) break;
             if (!pa_item(p, ustart, i, it) || it.n == 0) continue;
+            const int* own_table = a.table + (size_t)max(it.b, 0) * a.table_ld;
+            auto load_ids = [&](int t) {
+                if (t >= it.n || lane >= npg) return -2;
+                const PaTile kt = pa_tile(p, it, t);
+                const int key = kt.k0 + (lane << min(lps, 7));
+                if (key >= kt.hi || key + min(ps, kPaKeys) <= kt.lo) return -2;  // nothing of it is seen
+                return (kt.prefix ? a.prefix_table : own_table)[key >> lps];
+            };
+            // the ids of tile t become known to the issuing lanes, its masks to everyone
+            auto put_ids = [&](int t, int id) {
+                const bool have = id >= 0 && id < a.pool.n_pages;
+                if (!have && id != -2) set_dev_error(p.err, DEV_ERR_BAD_ARG);
+                if (lane < npg) ctl->pages[(tiles + t) & 15][lane] = have ? id : -1;
+                const uint32_t got = __ballot_sync(0xffffffffu, have);
+                if (lane < 2) {
+                    uint32_t m = 0;  // 16-key groups 4 lane .. 4 lane + 3
+#pragma unroll
+                    for (int q = 0; q < 4; ++q) m |= (got >> (((4 * lane + q) * 16) >> min(lps, 7)) & 1) << q;
+                    const PaTile kt = pa_tile(p, it, t);
+                    const int k0 = kt.k0 + lane * 64;
+                    ctl->okmask[(tiles + t) & 15][lane] = m | ((k0 < kt.lo || k0 + 64 > kt.hi || m != 0xFu) ? 256u : 0u);
+                }
+                __syncwarp();
+            };
+            auto issue = [&](bool v, int t, int h) {
+                const int st = pos % NST;
+                if (pos >= NST && !pa_wait_warp(&ctl->empty[st], (pos / NST - 1) & 1, ctl, p.err, DEV_ERR_EMPTY_WAIT)) {
+                    ok = false;
+                    return;
+                }
+                int page = -1, row = 0;
+                if (issues) {
+                    page = ctl->pages[(tiles + t) & 15][lps <= 6 ? h * nb + g : 0];
+                    if (lps > 6) row = (pa_tile(p, it, t).k0 & (ps - 1)) + h * 64;
+                }
+                const uint32_t got = __ballot_sync(0xffffffffu, page >= 0);
+                if (lane == 0) {
+                    mbar_arrive_expect_tx(&ctl->full[st], __popc(got) * box_bytes);
+                    if (v) {
+                        const uint32_t m = ctl->okmask[(tiles + t) & 15][h];
+                        if (m & 256u) {
+                            const PaTile kt = pa_tile(p, it, t);
+                            const int k0 = kt.k0 + h * 64;
+                            const int l0 = min(max(kt.lo - k0, 0), 64), h0 = min(max(kt.hi - k0, 0), 64);
+                            ctl->fix[fixes & 15] = make_int4(st, (pos / NST) & 1, l0, h0 | (int)((m & 0xFu) << 16));
+                            mbar_arrive(&ctl->fq[fixes & 15]);
+                            ++fixes;
+                        }
+                    }
+                }
+                __syncwarp();
+                if (page >= 0) tma_4d(dst0 + st * STAGE, v ? &p.tv : &p.tk, j * 64, row, it.kvh, page, &ctl->full[st]);
+                ++pos;
+            };
+            const int D = it.pair ? 1 : 2;
+            int ids = load_ids(0);
             if (nq > 0 && !pa_wait_warp(&ctl->qempty, (nq - 1) & 1, ctl, p.err, DEV_ERR_EMPTY_WAIT)) break;
             if (lane == 0) {
                 const int nslot = it.pair ? 2 : 1;
@@ -502,93 +610,86 @@ __global__ void __launch_bounds__(kPaThreads, 1) k_pattn(const __grid_constant__
                         tma_3d(qs + s * TILE + h * kPaHalf, &p.tq, h * 64, it.kvh * G, it.tok0 + s * p.TPT, &ctl->qfull);
             }
             ++nq;
-            for (int t = 0; t < it.n; ++t) {
-                const PaTile kt = pa_tile(p, it, t);
-                // lane g < npg: page g of the tile
-                const int key = kt.k0 + lane * box;
-                const bool want = lane < npg && key < kt.hi && key + box > kt.lo;
-                int page = -1;
-                if (want) page = kt.prefix ? a.prefix_table[key / ps] : a.table[(size_t)it.b * a.table_ld + key / ps];
-                const bool have = want && page >= 0 && page < a.pool.n_pages;
-                if (want && !have) set_dev_error(p.err, DEV_ERR_BAD_ARG);
-                const uint32_t got = __ballot_sync(0xffffffffu, have);
-                uint32_t mask = 0;  // bits of 16-key groups
-                for (int g = 0; g < npg; ++g)
-                    if (got >> g & 1) mask |= ((1u << (box / 16)) - 1) << (g * (box / 16));
-#pragma unroll
-                for (int kv = 0; kv < 2; ++kv) {
-                    const int st = pos % NST;
-                    if (pos >= NST && !pa_wait_warp(&ctl->empty[st], (pos / NST - 1) & 1, ctl, p.err, DEV_ERR_EMPTY_WAIT)) {
-                        ok = false;
-                        break;
-                    }
-                    if (lane == 0) {
-                        if (kv == 0) ctl->okmask[(pos >> 1) & 15] = mask;
-                        mbar_arrive_expect_tx(&ctl->full[st], __popc(got) * page_bytes);
-                    }
-                    __syncwarp();
-                    if (have)
-                        for (int h = 0; h < NH; ++h)
-                            tma_4d(kvs + st * TILE + h * kPaHalf + lane * box * 128, kv ? &p.tv : &p.tk, h * 64, key & (ps - 1), it.kvh,
-                                   page, &ctl->full[st]);
-                    ++pos;
-                }
-                if (!ok) break;
+            for (int t = 0; t < D && t < it.n && ok; ++t) {
+                put_ids(t, ids);
+                ids = load_ids(t + 1);
+                issue(false, t, 0);
+                if (ok) issue(false, t, 1);
             }
+            for (int t = 0; t < it.n && ok; ++t) {
+                const int tn = t + D;
+                if (tn < it.n) {
+                    put_ids(tn, ids);
+                    ids = load_ids(tn + 1);  // one tile ahead, so that a stage is refilled as soon as it is free
+                }
+#pragma unroll
+                for (int h = 0; h < 2; ++h) {
+                    issue(true, t, h);
+                    if (ok && tn < it.n) issue(false, tn, h);
+                    if (!ok) break;
+                }
+            }
+            tiles += it.n;
+        }
+        if (lane == 0) {  // the zeroing warp may go
+            ctl->fix[fixes & 15] = make_int4(-1, 0, 0, 0);
+            mbar_arrive(&ctl->fq[fixes & 15]);
         }
         // no copy may still be landing when the CTA exits
         for (uint32_t q = pos > NST ? pos - NST : 0; q < pos; ++q) mbar_wait(&ctl->full[q % NST], (q / NST) & 1);
         if (nq > 0) mbar_wait(&ctl->qfull, (nq - 1) & 1);
     } else if (warp == 9) {
         // ---------------- MMA issue: the warp walks together, one elected lane issues ----------------
-        constexpr uint32_t id_s = idesc_f16(BF, kPaKeys, false), id_o = idesc_f16(BF, HD, true);
+        constexpr uint32_t id_s = idesc_f16(BF, kPaKeys / 2, false), id_o = idesc_f16(BF, HD, true);
         const bool leader = elect_one();
-        uint32_t pos = 0, fixes = 0, np[2] = {0, 0};
+        uint32_t pos = 0, fixes = 0, tiles = 0, np[2] = {0, 0};
         int nq = 0;
         bool ok = true;
-        auto wait_k = [&](uint32_t q) {
-            ok = ok && pa_wait_warp(&ctl->full[q % NST], (q / NST) & 1, ctl, p.err, DEV_ERR_FULL_WAIT);
+        // the next stage of the ring
+        auto wait_stage = [&]() {
+            ok = ok && pa_wait_warp(&ctl->full[pos % NST], (pos / NST) & 1, ctl, p.err, DEV_ERR_FULL_WAIT);
         };
         auto commit = [&](uint64_t* bar) {
             if (leader) pa_commit(bar);
         };
-        auto score = [&](int slot, int qt, uint32_t q) {
-            pa_fence_after();
-            const uint32_t qa = sw128_lo(qs + qt * TILE, 16), ka = sw128_lo(kvs + (q % NST) * TILE, 16), d = tmem + slot * 128;
+        auto release = [&]() {
+            commit(&ctl->empty[pos % NST]);
+            ++pos;
+        };
+        // S of 64 keys: half h of slot's next tile, K in the current stage, against Q tile qt
+        auto score = [&](int slot, int h, int qt) {
+            const uint32_t qa = sw128_lo(qs + qt * TILE, 16), ka = sw128_lo(kvs + (pos % NST) * STAGE, 16);
+            const uint32_t d = tmem + slot * 128 + h * 64;
             if (leader) {
 #pragma unroll
-                for (int ks = 0; ks < HD / 16; ++ks) {
-                    const uint32_t o = ((ks >> 2) * kPaHalf + (ks & 3) * 32) >> 4;
-                    mma_ss(d, qa + o, ka + o, id_s, ks > 0);
-                }
-                pa_commit(&ctl->sfull[slot]);
+                for (int ks = 0; ks < HD / 16; ++ks)
+                    mma_ss(d, qa + (((ks >> 2) * kPaHalf + (ks & 3) * 32) >> 4), ka + (((ks >> 2) * kSHalf + (ks & 3) * 32) >> 4), id_s,
+                           ks > 0);
+                pa_commit(&ctl->sfull[slot][h]);
             }
         };
-        auto wait_v = [&](const PaItem& it, int t, uint32_t q) {
-            wait_k(q);
+        // V of half h of tile t in the current stage, its unseen rows zero
+        auto wait_v = [&](int t, int h) {
+            wait_stage();
+            if (ok && (*(volatile uint32_t*)&ctl->okmask[(tiles + t) & 15][h] & 256u)) {
+                ok = pa_wait_warp(&ctl->fixed[pos % NST], fixes >> (pos % NST) & 1, ctl, p.err, DEV_ERR_FULL_WAIT);
+                fixes ^= 1u << (pos % NST);
+            }
+        };
+        // O += P V over 64 keys (V in the current stage), once their P is there
+        auto value = [&](int slot, int h, bool acc, bool last) {
+            const uint32_t va = sw128_lo(kvs + (pos % NST) * STAGE, kSHalf);
+            const uint32_t d = tmem + 256 + slot * HD, pa = tmem + slot * 128 + h * 64;
+            ok = ok && pa_wait_warp(&ctl->pready[slot][h], np[slot] & 1, ctl, p.err, DEV_ERR_FULL_WAIT);
             if (!ok) return;
-            const PaTile kt = pa_tile(p, it, t);
-            const int st = q % NST;
-            if (kt.k0 < kt.lo || kt.k0 + kPaKeys > kt.hi || ctl->okmask[(q >> 1) & 15] != 0xFFu) {
-                ok = pa_wait_warp(&ctl->fixed[st], fixes >> st & 1, ctl, p.err, DEV_ERR_FULL_WAIT);
-                fixes ^= 1u << st;
-            }
-        };
-        // O += P V, the first half of the keys while the softmax still computes the second
-        auto value = [&](int slot, bool acc, uint32_t q) {
-            const uint32_t va = sw128_lo(kvs + (q % NST) * TILE, kPaHalf), d = tmem + 256 + slot * HD, pa = tmem + slot * 128;
+            pa_fence_after();
+            if (leader) {
 #pragma unroll
-            for (int h = 0; h < 2; ++h) {
-                ok = ok && pa_wait_warp(&ctl->pready[slot][h], np[slot] & 1, ctl, p.err, DEV_ERR_FULL_WAIT);
-                if (!ok) return;
-                pa_fence_after();
-                if (leader) {
-#pragma unroll
-                    for (int ks = 4 * h; ks < 4 * h + 4; ++ks) mma_ts(d, pa + ks * 8, va + ks * (2048 >> 4), id_o, acc || ks > 0);
-                    if (h == 1) pa_commit(&ctl->ofull[slot]);
-                }
+                for (int ks = 0; ks < 4; ++ks) mma_ts(d, pa + ks * 8, va + ks * (2048 >> 4), id_o, acc || h > 0 || ks > 0);
+                pa_commit(&ctl->ofull[slot]);
+                if (last && h == 1) pa_commit(&ctl->odone[slot]);
             }
-            ++np[slot];
+            if (h == 1) ++np[slot];
         };
         for (int k = 0;; ++k) {
             PaItem it;
@@ -597,60 +698,77 @@ __global__ void __launch_bounds__(kPaThreads, 1) k_pattn(const __grid_constant__
             if (!pa_item(p, ustart, i, it) || it.n == 0) continue;
             ok = pa_wait_warp(&ctl->qfull, nq & 1, ctl, p.err, DEV_ERR_FULL_WAIT);
             ++nq;
-            const uint32_t k0 = pos;
             const int n = it.n;
-            pos += 2 * n;
-            wait_k(k0);
-            if (!ok) break;
+            // Half tiles of K and V go through the ring in the order of their use: K of the first tile (of the first two of a
+            // single item, one per slot), then V of tile t and K of the tile that follows it on its slot, half by half.
+            // Each 64-key half of a slot's tile is a buffer of its own: its next S follows its product at once, while the
+            // softmax is at the other half (and the other slot).
             if (it.pair) {
-                score(0, 0, k0);
-                score(1, 1, k0);
-                commit(&ctl->empty[k0 % NST]);
-                if (n == 1) commit(&ctl->qempty);
+#pragma unroll
+                for (int h = 0; h < 2; ++h) {
+                    wait_stage();
+                    if (!ok) break;
+                    score(0, h, 0);
+                    score(1, h, 1);
+                    release();
+                }
+                if (n == 1 && ok) commit(&ctl->qempty);
                 for (int t = 0; t < n && ok; ++t) {
-                    const uint32_t v = k0 + 2 * t + 1, kn = v + 1;
-                    wait_v(it, t, v);
-                    value(0, t > 0, v);
-                    if (!ok) break;
-                    if (t + 1 < n) {
-                        wait_k(kn);
+                    const bool more = t + 1 < n;
+#pragma unroll
+                    for (int h = 0; h < 2; ++h) {
+                        // V is in the current stage, K of the next tile in the one behind it
+                        wait_v(t, h);
+                        value(0, h, t > 0, !more);
                         if (!ok) break;
-                        score(0, 0, kn);
+                        if (more) {
+                            ++pos;
+                            wait_stage();
+                            if (!ok) break;
+                            score(0, h, 0);
+                            --pos;
+                        }
+                        value(1, h, t > 0, !more);
+                        if (!ok) break;
+                        release();
+                        if (more) {
+                            score(1, h, 1);
+                            release();
+                        }
                     }
-                    value(1, t > 0, v);
-                    if (!ok) break;
-                    commit(&ctl->empty[v % NST]);
-                    if (t + 1 < n) {
-                        score(1, 1, kn);
-                        commit(&ctl->empty[kn % NST]);
-                        if (t + 2 == n) commit(&ctl->qempty);
-                    }
+                    if (t + 2 == n && ok) commit(&ctl->qempty);
                 }
             } else {
-                score(0, 0, k0);
-                commit(&ctl->empty[k0 % NST]);
-                if (n > 1) {
-                    wait_k(k0 + 2);
-                    if (!ok) break;
-                    score(1, 0, k0 + 2);
-                    commit(&ctl->empty[(k0 + 2) % NST]);
-                }
-                if (n <= 2) commit(&ctl->qempty);
-                for (int t = 0; t < n && ok; ++t) {
-                    const uint32_t v = k0 + 2 * t + 1, kn = v + 3;
-                    wait_v(it, t, v);
-                    value(t & 1, t > 1, v);
-                    if (!ok) break;
-                    commit(&ctl->empty[v % NST]);
-                    if (t + 2 < n) {
-                        wait_k(kn);
+#pragma unroll
+                for (int s = 0; s < 2; ++s)
+#pragma unroll
+                    for (int h = 0; h < 2; ++h) {
+                        if (s >= n || !ok) break;
+                        wait_stage();
                         if (!ok) break;
-                        score(t & 1, 0, kn);
-                        commit(&ctl->empty[kn % NST]);
-                        if (t + 3 == n) commit(&ctl->qempty);
+                        score(s, h, 0);
+                        release();
                     }
+                if (n <= 2 && ok) commit(&ctl->qempty);
+                for (int t = 0; t < n && ok; ++t) {
+                    const bool more = t + 2 < n;
+#pragma unroll
+                    for (int h = 0; h < 2; ++h) {
+                        wait_v(t, h);
+                        value(t & 1, h, t > 1, !more);
+                        if (!ok) break;
+                        release();
+                        if (more) {
+                            wait_stage();
+                            if (!ok) break;
+                            score(t & 1, h, 0);
+                            release();
+                        }
+                    }
+                    if (t + 3 == n && ok) commit(&ctl->qempty);
                 }
             }
+            tiles += n;
             if (!ok) break;
         }
         // every MMA issued above has completed before the tensor memory is released
@@ -659,42 +777,27 @@ __global__ void __launch_bounds__(kPaThreads, 1) k_pattn(const __grid_constant__
         __syncwarp();
     } else if (warp == 10) {
         // ---------------- V rows that no row of the item may see become zero ----------------
-        uint32_t pos = 0;
-        bool ok = true;
-        for (int k = 0; ok; ++k) {
-            PaItem it;
-            const int i = pa_next(ctl, k, lane, p.err);
-            if (i < 0) break;
-            if (!pa_item(p, ustart, i, it) || it.n == 0) continue;
-            for (int t = 0; t < it.n && ok; ++t) {
-                const PaTile kt = pa_tile(p, it, t);
-#pragma unroll
-                for (int kv = 0; kv < 2; ++kv) {
-                    const int st = pos % NST;
-                    ok = ok && pa_wait_warp(&ctl->full[st], (pos / NST) & 1, ctl, p.err, DEV_ERR_FULL_WAIT);
-                    if (!ok) break;
-                    if (kv) {
-                        const uint32_t mask = ctl->okmask[(pos >> 1) & 15];
-                        if (kt.k0 < kt.lo || kt.k0 + kPaKeys > kt.hi || mask != 0xFFu) {
-                            // 8 lanes a row (16 bytes each of 128), 4 rows at a time
-                            for (int r = lane >> 3; r < kPaKeys; r += 4)
-                                if (kt.k0 + r < kt.lo || kt.k0 + r >= kt.hi || !(mask >> (r >> 4) & 1))
-                                    for (int h = 0; h < NH; ++h)
-                                        asm volatile("st.shared.v4.u32 [%0], {%1, %1, %1, %1};" ::"r"(
-                                                         kvs + st * TILE + h * kPaHalf + r * 128 + (lane & 7) * 16),
-                                                     "r"(0)
-                                                     : "memory");
-                            asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-                            __syncwarp();
-                            if (lane == 0) mbar_arrive(&ctl->fixed[st]);
-                        }
-                    }
-                    if (lane == 0) mbar_arrive(&ctl->empty[st]);
-                    ++pos;
-                }
-            }
+        for (uint32_t r = 0;; ++r) {
+            // no request may come for long; the TMA warp always posts the last one, and itself waits for 2 s at most
+            bool there = false;
+            for (int n = 0; n < 1024 && !there && !*(volatile int*)&ctl->abort; ++n)
+                there = __all_sync(0xffffffffu, mbar_wait(&ctl->fq[r & 15], r >> 4 & 1));
+            if (!there) break;
+            const int4 f = ctl->fix[r & 15];
+            if (f.x < 0 || !pa_wait_warp(&ctl->full[f.x], f.y, ctl, p.err, DEV_ERR_FULL_WAIT)) break;
+            const int hi = f.w & 0xFFFF;
+            // 8 lanes a row (16 bytes each of 128), 4 rows at a time
+            for (int q = lane >> 3; q < 64; q += 4)
+                if (q < f.z || q >= hi || !(f.w >> (16 + (q >> 4)) & 1))
+                    for (int h = 0; h < NH; ++h)
+                        asm volatile("st.shared.v4.u32 [%0], {%1, %1, %1, %1};" ::"r"(kvs + f.x * STAGE + h * kSHalf + q * 128 + (lane & 7) * 16),
+                                     "r"(0)
+                                     : "memory");
+            asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&ctl->fixed[f.x]);
         }
-    } else {
+    } else if (warp == 11) {
         // ---------------- scheduler ----------------
         // The grid has one CTA per item; a running CTA takes over CTAs that have not started (cluster launch
         // control), so unequal items even out over the SMs and set-up is paid once per SM.
@@ -731,19 +834,17 @@ __global__ void __launch_bounds__(kPaThreads, 1) k_pattn(const __grid_constant__
             }
         }
         __syncwarp();
-    }
     } else {
-        asm volatile("setmaxnreg.inc.sync.aligned.u32 216;");
         // ---------------- softmax: thread = row of its slot ----------------
         const int slot = warp >> 2, row = tid & 127;
         const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;
-        const uint32_t ts = tmem + lanes + slot * 128, to = tmem + lanes + 256 + slot * HD;
+        const uint32_t ts0 = tmem + lanes + slot * 128, to = tmem + lanes + 256 + slot * HD;
         const int row_tok = row / G, row_head = row - row_tok * G;
         const float kLog2e = 1.4426950408889634f;
         const float sc2 = a.scale * kLog2e;
         // capped: cap log2e tanh(x) with x = scale s / cap, as cap log2e (1 - 2 / (1 + 2^(2 log2e x)))
-        const float cap2 = a.softcap * kLog2e, xs = a.softcap > 0.f ? 2.f * kLog2e * a.scale / a.softcap : 0.f;
-        uint32_t ns = 0, no = 0, nm = 0, tiles = 0;
+        const float cap2 = a.softcap * kLog2e, x1 = a.softcap > 0.f ? a.scale / a.softcap : 0.f;
+        uint32_t ns = 0, np = 0, nd = 0, nm = 0, tiles = 0;  // phases of sfull, ofull, odone and the merges; key tiles so far
         bool ok = true;
         for (int k = 0; ok; ++k) {
             PaItem it;
@@ -776,124 +877,154 @@ __global__ void __launch_bounds__(kPaThreads, 1) k_pattn(const __grid_constant__
             const bool idle = !__any_sync(0xffffffffu, live);
             float m = -INFINITY, l = 0.f;
             const int step = it.pair ? 1 : 2;
-            bool first = true;
-            for (int t = it.pair ? 0 : slot; t < it.n; t += step) {
+            uint32_t no = 0;  // products of this item
+            for (int t = it.pair ? 0 : slot; t < it.n && ok; t += step, ++ns) {
                 const PaTile kt = pa_tile(p, it, t);
-                const int lo = (kt.prefix ? lo_p : lo_o) - kt.k0, hi = (kt.prefix ? hi_p : hi_o) - kt.k0;
-                ok = pa_wait_warp(&ctl->sfull[slot], ns & 1, ctl, p.err, DEV_ERR_FULL_WAIT);
-                ++ns;
-                if (!ok) break;
-                if (idle) {
-                    mbar_arrive(&ctl->pready[slot][0]);
-                    mbar_arrive(&ctl->pready[slot][1]);
-                    ++no;
-                    first = false;
-                    continue;
-                }
-                pa_fence_after();
-                uint32_t y[4][32];
-#pragma unroll
-                for (int c = 0; c < 4; ++c) pa_ld32(ts + c * 32, y[c]);
-#pragma unroll
-                for (int c = 0; c < 4; ++c) pa_wait_ld(y[c]);
-                if (MOD) {
-                    if (a.softcap > 0.f) {
-#pragma unroll
-                        for (int c = 0; c < 4; ++c)
-#pragma unroll
-                            for (int e = 0; e < 32; ++e)
-                                y[c][e] = __float_as_uint(
-                                    fmaf(rcp(1.f + ex2(__uint_as_float(y[c][e]) * xs)), -2.f * cap2, cap2));
-                    } else {
-#pragma unroll
-                        for (int c = 0; c < 4; ++c)
-#pragma unroll
-                            for (int e = 0; e < 32; ++e) y[c][e] = __float_as_uint(__uint_as_float(y[c][e]) * sc2);
-                    }
-                    if (a.alibi) {
-                        const float bias = slope * (float)((kt.prefix ? P : 0) + own - kt.k0);
-#pragma unroll
-                        for (int c = 0; c < 4; ++c)
-#pragma unroll
-                            for (int e = 0; e < 32; ++e)
-                                y[c][e] = __float_as_uint(__uint_as_float(y[c][e]) + fmaf(slope, (float)(c * 32 + e), -bias));
-                    }
-                }
-                const uint32_t mask = *(volatile uint32_t*)&ctl->okmask[(tiles + t) & 15];
-                if (!__all_sync(0xffffffffu, lo <= 0 && hi >= kPaKeys && mask == 0xFFu)) {
-#pragma unroll
-                    for (int c = 0; c < 4; ++c) {
-                        // keys of this quarter: bits [lo, hi) of those that were loaded
-                        const int l0 = min(max(lo - c * 32, 0), 32), h0 = min(max(hi - c * 32, 0), 32);
-                        uint32_t vis = (h0 < 32 ? (1u << h0) - 1u : 0xffffffffu) & ~(l0 < 32 ? (1u << l0) - 1u : 0xffffffffu);
-                        if (!(mask >> (2 * c) & 1)) vis &= 0xffff0000u;
-                        if (!(mask >> (2 * c + 1) & 1)) vis &= 0x0000ffffu;
-#pragma unroll
-                        for (int e = 0; e < 32; ++e)
-                            if (!(vis & (1u << e))) y[c][e] = 0xff800000u;  // -infinity
-                    }
-                }
-                float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
-#pragma unroll
-                for (int c = 0; c < 4; ++c)
-#pragma unroll
-                    for (int e = 0; e < 32; e += 2)
-                        mx[(e >> 1) & 3] = fmaxf(mx[(e >> 1) & 3], fmaxf(__uint_as_float(y[c][e]), __uint_as_float(y[c][e + 1])));
-                float top = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3]));
-                if (!MOD) top *= sc2;
-                float factor = 1.f;
-                if (top > m + kSlack || (m == -INFINITY && top != -INFINITY)) {
-                    factor = ex2(m - top);  // 0 from a maximum of -infinity
-                    m = top;
-                }
-                l *= factor;
-                if (__any_sync(0xffffffffu, factor != 1.f) && !first) {
-                    // O of the tiles so far refers to the old maximum
-                    ok = pa_wait_warp(&ctl->ofull[slot], (no - 1) & 1, ctl, p.err, DEV_ERR_FULL_WAIT);
-                    if (!ok) break;
-                    pa_fence_after();
-#pragma unroll
-                    for (int c = 0; c < HD / 32; ++c) {
-                        uint32_t o[32];
-                        pa_ld32(to + c * 32, o);
-                        pa_wait_ld(o);
-#pragma unroll
-                        for (int e = 0; e < 32; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * factor);
-                        pa_st32(to + c * 32, o);
-                    }
-                }
-                const float ref = (m == -INFINITY ? 0.f : m) - kShift;
-                const float2 ref2 = make_float2(-ref, -ref), one2 = make_float2(MOD ? 1.f : sc2, MOD ? 1.f : sc2);
-                float2 sum[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
-#pragma unroll
+#pragma unroll 1
                 for (int h = 0; h < 2; ++h) {
-                    uint32_t pk[32];
+                    ok = pa_wait_warp(&ctl->sfull[slot][h], ns & 1, ctl, p.err, DEV_ERR_FULL_WAIT);
+                    if (!ok) break;
+                    if (!idle) {
+                        pa_fence_after();
+                        const uint32_t ts = ts0 + h * 64;
+                        uint32_t y[2][32];
+                        pa_ld32(ts, y[0]);
+                        pa_ld32(ts + 32, y[1]);
+                        const int k0 = kt.k0 + h * 64;
+                        const int lo = (kt.prefix ? lo_p : lo_o) - k0, hi = (kt.prefix ? hi_p : hi_o) - k0;
+                        const uint32_t mask = *(volatile uint32_t*)&ctl->okmask[(tiles + t) & 15][h] & 0xFu;
+                        const bool whole = __all_sync(0xffffffffu, lo <= 0 && hi >= 64 && mask == 0xFu);
+                        pa_wait_ld(y[0]);
+                        pa_wait_ld(y[1]);
+                        if (MOD) {
+                            if (a.softcap > 0.f) {
+                                // scores below the cap (nearly all): tanh without the special function unit, which the
+                                // weights' exp2 already fills
+                                float big = 0.f;
 #pragma unroll
-                    for (int e = 0; e < 32; ++e) {
-                        const int c = h * 2 + (e >> 4), x = (e & 15) * 2;
-                        float2 z = __ffma2_rn(make_float2(__uint_as_float(y[c][x]), __uint_as_float(y[c][x + 1])), one2, ref2);
-                        z.x = ex2(z.x);
-                        z.y = ex2(z.y);
-                        sum[e & 1] = __fadd2_rn(sum[e & 1], z);
-                        pk[e] = pa_pack<T>(z.x, z.y);
+                                for (int c = 0; c < 2; ++c)
+#pragma unroll
+                                    for (int e = 0; e < 32; e += 2)
+                                        big = fmaxf(big, fmaxf(fabsf(__uint_as_float(y[c][e])), fabsf(__uint_as_float(y[c][e + 1]))));
+                                if (__all_sync(0xffffffffu, big * fabsf(x1) <= 1.f)) {
+#pragma unroll
+                                    for (int c = 0; c < 2; ++c)
+#pragma unroll
+                                        for (int e = 0; e < 32; e += 2) {
+                                            const float2 x = __fmul2_rn(make_float2(__uint_as_float(y[c][e]), __uint_as_float(y[c][e + 1])),
+                                                                        make_float2(x1, x1));
+                                            const float2 z = __fmul2_rn(tanh_small(x), make_float2(cap2, cap2));
+                                            y[c][e] = __float_as_uint(z.x);
+                                            y[c][e + 1] = __float_as_uint(z.y);
+                                        }
+                                } else {  // the same choice for each score, whatever its neighbours are
+#pragma unroll
+                                    for (int c = 0; c < 2; ++c)
+#pragma unroll
+                                        for (int e = 0; e < 32; e += 2) {
+                                            const float2 x = __fmul2_rn(make_float2(__uint_as_float(y[c][e]), __uint_as_float(y[c][e + 1])),
+                                                                        make_float2(x1, x1));
+                                            float2 z = __fmul2_rn(tanh_small(x), make_float2(cap2, cap2));
+                                            if (!(fabsf(x.x) <= 1.f)) z.x = fmaf(rcp(1.f + ex2(x.x * (2.f * kLog2e))), -2.f * cap2, cap2);
+                                            if (!(fabsf(x.y) <= 1.f)) z.y = fmaf(rcp(1.f + ex2(x.y * (2.f * kLog2e))), -2.f * cap2, cap2);
+                                            y[c][e] = __float_as_uint(z.x);
+                                            y[c][e + 1] = __float_as_uint(z.y);
+                                        }
+                                }
+                            } else {
+#pragma unroll
+                                for (int c = 0; c < 2; ++c)
+#pragma unroll
+                                    for (int e = 0; e < 32; ++e) y[c][e] = __float_as_uint(__uint_as_float(y[c][e]) * sc2);
+                            }
+                            if (a.alibi) {
+                                const float bias = slope * (float)((kt.prefix ? P : 0) + own - k0);
+#pragma unroll
+                                for (int c = 0; c < 2; ++c)
+#pragma unroll
+                                    for (int e = 0; e < 32; ++e)
+                                        y[c][e] = __float_as_uint(__uint_as_float(y[c][e]) + fmaf(slope, (float)(c * 32 + e), -bias));
+                            }
+                        }
+                        if (!whole) {
+#pragma unroll
+                            for (int c = 0; c < 2; ++c) {
+                                // these 32 keys: bits [lo, hi) of those that were loaded
+                                const int l0 = min(max(lo - c * 32, 0), 32), h0 = min(max(hi - c * 32, 0), 32);
+                                uint32_t vis = (h0 < 32 ? (1u << h0) - 1u : 0xffffffffu) & ~(l0 < 32 ? (1u << l0) - 1u : 0xffffffffu);
+                                if (!(mask >> (2 * c) & 1)) vis &= 0xffff0000u;
+                                if (!(mask >> (2 * c + 1) & 1)) vis &= 0x0000ffffu;
+#pragma unroll
+                                for (int e = 0; e < 32; ++e)
+                                    if (!(vis & (1u << e))) y[c][e] = 0xff800000u;  // -infinity
+                            }
+                        }
+                        float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll
+                        for (int c = 0; c < 2; ++c)
+#pragma unroll
+                            for (int e = 0; e < 32; e += 2)
+                                mx[(e >> 1) & 3] = fmaxf(mx[(e >> 1) & 3], fmaxf(__uint_as_float(y[c][e]), __uint_as_float(y[c][e + 1])));
+                        float top = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3]));
+                        if (!MOD) top *= sc2;
+                        const bool rise = top > m + kSlack || (m == -INFINITY && top != -INFINITY);
+                        if (__any_sync(0xffffffffu, rise)) {
+                            const float factor = rise ? ex2(m - top) : 1.f;  // 0 from a maximum of -infinity
+                            if (rise) m = top;
+                            l *= factor;
+                            if (no > 0) {
+                                // O of the keys so far refers to the old maximum
+                                ok = pa_wait_warp(&ctl->ofull[slot], (np + no - 1) & 1, ctl, p.err, DEV_ERR_FULL_WAIT);
+                                if (!ok) break;
+                                pa_fence_after();
+#pragma unroll 1
+                                for (int c = 0; c < HD / 32; ++c) {
+                                    uint32_t o[32];
+                                    pa_ld32(to + c * 32, o);
+                                    pa_wait_ld(o);
+#pragma unroll
+                                    for (int e = 0; e < 32; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * factor);
+                                    pa_st32(to + c * 32, o);
+                                }
+                            }
+                        }
+                        const float ref = (m == -INFINITY ? 0.f : m) - kShift;
+                        const float2 ref2 = make_float2(-ref, -ref), one2 = make_float2(MOD ? 1.f : sc2, MOD ? 1.f : sc2);
+                        float2 sum[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
+                        uint32_t pk[32];
+#pragma unroll
+                        for (int e = 0; e < 32; ++e) {
+                            float2 z = __ffma2_rn(make_float2(__uint_as_float(y[e >> 4][(e & 15) * 2]), __uint_as_float(y[e >> 4][(e & 15) * 2 + 1])),
+                                                  one2, ref2);
+                            if (POLY && e % (POLY ? POLY : 1) == POLY - 1) {
+                                z = ex2_fma(z);
+                            } else {
+                                z.x = ex2(z.x);
+                                z.y = ex2(z.y);
+                            }
+                            sum[e & 1] = __fadd2_rn(sum[e & 1], z);
+                            pk[e] = pa_pack<T>(z.x, z.y);
+                        }
+                        pa_st32(ts, pk);
+                        l += (sum[0].x + sum[0].y) + (sum[1].x + sum[1].y);
+                        pa_wait_st();
+                        pa_fence_before();
                     }
-                    pa_st32(ts + h * 32, pk);
-                    pa_wait_st();
-                    pa_fence_before();
-                    mbar_arrive(&ctl->pready[slot][h]);
+                    __syncwarp();
+                    if (lane == 0) mbar_arrive(&ctl->pready[slot][h]);
+                    ++no;
                 }
-                l += (sum[0].x + sum[0].y) + (sum[1].x + sum[1].y);
-                ++no;
-                first = false;
             }
             if (!ok) break;
             tiles += it.n;
             // ---- the item's result ----
-            if (!first) {
-                ok = pa_wait_warp(&ctl->ofull[slot], (no - 1) & 1, ctl, p.err, DEV_ERR_FULL_WAIT);
+            if (no > 0) {
+                ok = pa_wait_warp(&ctl->odone[slot], nd & 1, ctl, p.err, DEV_ERR_FULL_WAIT);
                 if (!ok) break;
                 pa_fence_after();
+                ++nd;
             }
+            np += no;
             float f0 = 1.f, f1 = 0.f;
             const bool merge = !it.pair && it.n > 1;
             if (merge) {
@@ -1127,7 +1258,7 @@ int run_tc(const sd_attn_args& a, int dev, cudaStream_t st) {
     for (int i = 0; i < 2; ++i) {
         const cuuint64_t dims[4] = {hd, (cuuint64_t)k.page_size, (cuuint64_t)k.n_kv_heads, (cuuint64_t)k.n_pages};
         const cuuint64_t strides[3] = {(cuuint64_t)k.pos_stride * 2, (cuuint64_t)k.head_stride * 2, (cuuint64_t)k.page_stride * 2};
-        const cuuint32_t box[4] = {64, (cuuint32_t)std::min(k.page_size, kPaKeys), 1, 1};
+        const cuuint32_t box[4] = {64, (cuuint32_t)std::min(k.page_size, kPaKeys / 2), 1, 1};
         const int rc = encode(i ? &p.tv : &p.tk, bf, 4, i ? k.v : k.k, dims, strides, box);
         if (rc) return rc;
     }

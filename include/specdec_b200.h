@@ -137,7 +137,7 @@ SD_API void sd_host_cache_clear(void);
  * of range is left out as each call says and records DEV error 3, which sd_device_error reads.
  * ====================================================================================== */
 enum { SD_F32 = 0, SD_F16 = 1, SD_BF16 = 2 };
-#define SD_PAGES_MAX_REQ 8192
+#define SD_PAGES_MAX_REQ 4096
 #define SD_PAGE_MIN 16
 #define SD_PAGE_MAX 256
 

@@ -57,7 +57,7 @@ def new_state(n_req, n_pages, ld):
 
 
 @pytest.mark.parametrize("n_req,page,max_len,n_pages,q_stride", [(1, 16, 100, 7, 0), (1, 256, 1, 1, 0), (7, 32, 500, 60, 0), (7, 16, 333, 40, 9),
-                                                                 (600, 16, 200, 4000, 0), (513, 64, 1000, 5000, 3), (8192, 16, 64, 20000, 0)])
+                                                                 (600, 16, 200, 4000, 0), (513, 64, 1000, 5000, 3), (4096, 16, 64, 10000, 0)])
 def test_plan_random_steps(pg, n_req, page, max_len, n_pages, q_stride):
     """Requests grow, shrink (rejected drafts), end and are replaced; some steps want more pages than there are."""
     rng = np.random.default_rng(n_req + page)

@@ -38,8 +38,8 @@ def refused(rc, word=None):
 
 
 @pytest.mark.parametrize("kw", [dict(table=None), dict(held=None), dict(free_pages=None), dict(n_free=None), dict(n_req=0),
-                                dict(n_req=8193), dict(table_ld=0), dict(n_pages=0), dict(page_size=8), dict(page_size=48),
-                                dict(page_size=512), dict(n_pages=1 << 28), dict(table_ld=1 << 28), dict(n_req=8192, table_ld=1 << 19)])
+                                dict(n_req=4097), dict(table_ld=0), dict(n_pages=0), dict(page_size=8), dict(page_size=48),
+                                dict(page_size=512), dict(n_pages=1 << 28), dict(table_ld=1 << 28), dict(n_req=4096, table_ld=1 << 20)])
 def test_pages_refusals(kw):
     L = _lib.lib()
     p = pages(**kw)
@@ -73,7 +73,7 @@ def test_append_refusals():
 
 
 @pytest.mark.parametrize("kw", [dict(q=None), dict(out=None), dict(table=None), dict(kv_len=None), dict(q_start=None), dict(q_len=None),
-                                dict(n_req=0), dict(n_req=9000), dict(n_heads=0), dict(n_heads=30), dict(n_heads=8 * 129), dict(max_kv=129),
+                                dict(n_req=0), dict(n_req=4097), dict(n_heads=0), dict(n_heads=30), dict(n_heads=8 * 129), dict(max_kv=129),
                                 dict(max_q=-1), dict(max_kv=-1), dict(n_tokens=-1), dict(prefix_len=-1), dict(prefix_len=16),
                                 dict(window=-1), dict(table_ld=0), dict(softcap=-1.0), dict(softcap=float("nan")),
                                 dict(scale=float("nan")), dict(q_head=64), dict(out_head=64),
