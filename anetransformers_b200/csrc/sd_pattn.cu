@@ -140,7 +140,7 @@ struct PaArgs {
 };
 
 struct PaCtl {
-    uint64_t qfull, qempty;
+    uint64_t qfull[2], qempty[2];  // per Q tile buffer
     uint64_t full[16], empty[16], fixed[16];
     uint64_t sfull[2][2], pready[2][2];  // [slot][half of the tile's keys]: S and P written
     // A parity wait tells a phase from its neighbour only: ofull (one phase per half's product) is waited for where the
@@ -304,10 +304,11 @@ __device__ __forceinline__ void tma_3d(uint32_t dst, const CUtensorMap* m, int x
         "l"(m), "r"(smem_u32(bar)), "r"(x), "r"(y), "r"(z)
         : "memory");
 }
-__device__ __forceinline__ void tma_4d(uint32_t dst, const CUtensorMap* m, int x, int y, int z, int w, uint64_t* bar) {
+__device__ __forceinline__ void tma_5d(uint32_t dst, const CUtensorMap* m, int x, int y, int z, int w, int v, uint64_t* bar) {
     asm volatile(
-        "cp.async.bulk.tensor.4d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5, %6}], [%2];" ::"r"(dst),
-        "l"(m), "r"(smem_u32(bar)), "r"(x), "r"(y), "r"(z), "r"(w)
+        "cp.async.bulk.tensor.5d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5, %6, %7}], [%2];" ::"r"(
+            dst),
+        "l"(m), "r"(smem_u32(bar)), "r"(x), "r"(y), "r"(z), "r"(w), "r"(v)
         : "memory");
 }
 
@@ -459,8 +460,10 @@ __global__ void __launch_bounds__(kPaThreads, 1) k_pattn(const __grid_constant__
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
 
     if (tid == 0) {
-        mbar_init(&ctl->qfull, 1);
-        mbar_init(&ctl->qempty, 1);
+        for (int i = 0; i < 2; ++i) {
+            mbar_init(&ctl->qfull[i], 1);
+            mbar_init(&ctl->qempty[i], 1);
+        }
         for (int i = 0; i < NST; ++i) {
             mbar_init(&ctl->full[i], 1);
             mbar_init(&ctl->empty[i], 1);
@@ -530,15 +533,18 @@ __global__ void __launch_bounds__(kPaThreads, 1) k_pattn(const __grid_constant__
 
     if (warp == 8) {
         // ---------------- TMA ----------------
-        uint32_t pos = 0, tiles = 0, fixes = 0;
-        int nq = 0;
-        const int lps = 31 - __clz(ps), box = min(ps, kPaKeys / 2), nb = kPaKeys / 2 / box;  // boxes per stage and 64 elements
+        // One TMA box has at most 64 rows of one page and 128-byte swizzle rows, so 64 elements; it takes the copy engine
+        // about 3.1 clk a row and 51 clk a box (measured from L2), so few boxes: both 64-element halves of V rows come in one
+        // ([page][half][row], which the product's descriptor can follow page by page), of K rows where a page fills a stage.
+        uint32_t pos = 0, tiles = 0, fixes = 0, nq[2] = {0, 0}, qb = 0;
+        const int lps = 31 - __clz(ps), box = min(ps, kPaKeys / 2), nb = kPaKeys / 2 / box;  // boxes per stage along the rows
         const int npg = kPaKeys / min(ps, kPaKeys);                                          // pages per tile
-        const uint32_t box_bytes = (uint32_t)box * 128u;
-        // lane NH g + j brings 64-element half j of box g of a stage; lane g < npg reads the id of page g of a tile
-        const int g = lane / NH, j = lane % NH;
-        const bool issues = g < nb;
-        const uint32_t dst0 = kvs + j * kSHalf + g * box * 128;
+        const int nhk = nb == 1 ? 1 : NH;                                                    // boxes of K along the row
+        const uint32_t page_bytes = (uint32_t)box * 128u * NH;
+        // lane nhk g + j brings part j of the K rows of box g of a stage, lane g the V rows; lane g < npg reads the id of
+        // page g of a tile
+        const int gk = lane / nhk, jk = lane % nhk;
+        const uint32_t dst_k = kvs + jk * kSHalf + gk * box * 128, dst_v = kvs + lane * page_bytes;
         bool ok = true;
         for (int k = 0; ok; ++k) {
             PaItem it;
@@ -570,19 +576,19 @@ __global__ void __launch_bounds__(kPaThreads, 1) k_pattn(const __grid_constant__
                 __syncwarp();
             };
             auto issue = [&](bool v, int t, int h) {
-                const int st = pos % NST;
+                const int st = pos % NST, g = v ? lane : gk;
                 if (pos >= NST && !pa_wait_warp(&ctl->empty[st], (pos / NST - 1) & 1, ctl, p.err, DEV_ERR_EMPTY_WAIT)) {
                     ok = false;
                     return;
                 }
                 int page = -1, row = 0;
-                if (issues) {
+                if (g < nb) {
                     page = ctl->pages[(tiles + t) & 15][lps <= 6 ? h * nb + g : 0];
                     if (lps > 6) row = (pa_tile(p, it, t).k0 & (ps - 1)) + h * 64;
                 }
                 const uint32_t got = __ballot_sync(0xffffffffu, page >= 0);
                 if (lane == 0) {
-                    mbar_arrive_expect_tx(&ctl->full[st], __popc(got) * box_bytes);
+                    mbar_arrive_expect_tx(&ctl->full[st], __popc(got) * (v || nhk == 1 ? page_bytes : page_bytes / NH));
                     if (v) {
                         const uint32_t m = ctl->okmask[(tiles + t) & 15][h];
                         if (m & 256u) {
@@ -596,20 +602,24 @@ __global__ void __launch_bounds__(kPaThreads, 1) k_pattn(const __grid_constant__
                     }
                 }
                 __syncwarp();
-                if (page >= 0) tma_4d(dst0 + st * STAGE, v ? &p.tv : &p.tk, j * 64, row, it.kvh, page, &ctl->full[st]);
+                if (page >= 0) tma_5d((v ? dst_v : dst_k) + st * STAGE, v ? &p.tv : &p.tk, 0, row, v ? 0 : jk, it.kvh, page, &ctl->full[st]);
                 ++pos;
             };
             const int D = it.pair ? 1 : 2;
             int ids = load_ids(0);
-            if (nq > 0 && !pa_wait_warp(&ctl->qempty, (nq - 1) & 1, ctl, p.err, DEV_ERR_EMPTY_WAIT)) break;
-            if (lane == 0) {
-                const int nslot = it.pair ? 2 : 1;
-                mbar_arrive_expect_tx(&ctl->qfull, (uint32_t)(nslot * NH * p.TPT * G * 128));
-                for (int s = 0; s < nslot; ++s)
+            // Q: both buffers for a pair; single items take turns, so that the next one's Q need not wait for this one
+            for (int s = 0; s < 2 && ok; ++s) {
+                if (!it.pair && s != (int)qb) continue;
+                ok = nq[s] == 0 || pa_wait_warp(&ctl->qempty[s], (nq[s] - 1) & 1, ctl, p.err, DEV_ERR_EMPTY_WAIT);
+                if (ok && lane == 0) {
+                    mbar_arrive_expect_tx(&ctl->qfull[s], (uint32_t)(NH * p.TPT * G * 128));
                     for (int h = 0; h < NH; ++h)
-                        tma_3d(qs + s * TILE + h * kPaHalf, &p.tq, h * 64, it.kvh * G, it.tok0 + s * p.TPT, &ctl->qfull);
+                        tma_3d(qs + s * TILE + h * kPaHalf, &p.tq, h * 64, it.kvh * G, it.tok0 + (it.pair ? s * p.TPT : 0), &ctl->qfull[s]);
+                }
+                nq[s] += ok;
             }
-            ++nq;
+            if (!it.pair) qb ^= 1;
+            if (!ok) break;
             for (int t = 0; t < D && t < it.n && ok; ++t) {
                 put_ids(t, ids);
                 ids = load_ids(t + 1);
@@ -637,13 +647,18 @@ __global__ void __launch_bounds__(kPaThreads, 1) k_pattn(const __grid_constant__
         }
         // no copy may still be landing when the CTA exits
         for (uint32_t q = pos > NST ? pos - NST : 0; q < pos; ++q) mbar_wait(&ctl->full[q % NST], (q / NST) & 1);
-        if (nq > 0) mbar_wait(&ctl->qfull, (nq - 1) & 1);
+        for (int s = 0; s < 2; ++s)
+            if (nq[s] > 0) mbar_wait(&ctl->qfull[s], (nq[s] - 1) & 1);
     } else if (warp == 9) {
         // ---------------- MMA issue: the warp walks together, one elected lane issues ----------------
         constexpr uint32_t id_s = idesc_f16(BF, kPaKeys / 2, false), id_o = idesc_f16(BF, HD, true);
         const bool leader = elect_one();
-        uint32_t pos = 0, fixes = 0, tiles = 0, np[2] = {0, 0};
-        int nq = 0;
+        // 16 keys of V further: within a box [64-element half][row] of up to 64 rows, or in the next page's
+        const uint32_t vbox = min(ps, kPaKeys / 2);
+        uint32_t vstep[4];
+#pragma unroll
+        for (int ks = 0; ks < 4; ++ks) vstep[ks] = (ks * 16 / vbox * vbox * 128 * NH + ks * 16 % vbox * 128) >> 4;
+        uint32_t pos = 0, fixes = 0, tiles = 0, np[2] = {0, 0}, nq[2] = {0, 0}, qb = 0;
         bool ok = true;
         // the next stage of the ring
         auto wait_stage = [&]() {
@@ -678,14 +693,14 @@ __global__ void __launch_bounds__(kPaThreads, 1) k_pattn(const __grid_constant__
         };
         // O += P V over 64 keys (V in the current stage), once their P is there
         auto value = [&](int slot, int h, bool acc, bool last) {
-            const uint32_t va = sw128_lo(kvs + (pos % NST) * STAGE, kSHalf);
+            const uint32_t va = sw128_lo(kvs + (pos % NST) * STAGE, vbox * 128);
             const uint32_t d = tmem + 256 + slot * HD, pa = tmem + slot * 128 + h * 64;
             ok = ok && pa_wait_warp(&ctl->pready[slot][h], np[slot] & 1, ctl, p.err, DEV_ERR_FULL_WAIT);
             if (!ok) return;
             pa_fence_after();
             if (leader) {
 #pragma unroll
-                for (int ks = 0; ks < 4; ++ks) mma_ts(d, pa + ks * 8, va + ks * (2048 >> 4), id_o, acc || h > 0 || ks > 0);
+                for (int ks = 0; ks < 4; ++ks) mma_ts(d, pa + ks * 8, va + vstep[ks], id_o, acc || h > 0 || ks > 0);
                 pa_commit(&ctl->ofull[slot]);
                 if (last && h == 1) pa_commit(&ctl->odone[slot]);
             }
@@ -696,8 +711,17 @@ __global__ void __launch_bounds__(kPaThreads, 1) k_pattn(const __grid_constant__
             const int i = pa_next(ctl, k, lane, p.err);
             if (i < 0) break;
             if (!pa_item(p, ustart, i, it) || it.n == 0) continue;
-            ok = pa_wait_warp(&ctl->qfull, nq & 1, ctl, p.err, DEV_ERR_FULL_WAIT);
-            ++nq;
+            const int q0 = it.pair ? 0 : (int)qb;
+            for (int s = q0; s <= (it.pair ? 1 : q0); ++s) {
+                ok = ok && pa_wait_warp(&ctl->qfull[s], nq[s] & 1, ctl, p.err, DEV_ERR_FULL_WAIT);
+                ++nq[s];
+            }
+            if (!it.pair) qb ^= 1;
+            if (!ok) break;
+            auto q_done = [&]() {
+                commit(&ctl->qempty[q0]);
+                if (it.pair) commit(&ctl->qempty[1]);
+            };
             const int n = it.n;
             // Half tiles of K and V go through the ring in the order of their use: K of the first tile (of the first two of a
             // single item, one per slot), then V of tile t and K of the tile that follows it on its slot, half by half.
@@ -712,7 +736,7 @@ __global__ void __launch_bounds__(kPaThreads, 1) k_pattn(const __grid_constant__
                     score(1, h, 1);
                     release();
                 }
-                if (n == 1 && ok) commit(&ctl->qempty);
+                if (n == 1 && ok) q_done();
                 for (int t = 0; t < n && ok; ++t) {
                     const bool more = t + 1 < n;
 #pragma unroll
@@ -736,7 +760,7 @@ __global__ void __launch_bounds__(kPaThreads, 1) k_pattn(const __grid_constant__
                             release();
                         }
                     }
-                    if (t + 2 == n && ok) commit(&ctl->qempty);
+                    if (t + 2 == n && ok) q_done();
                 }
             } else {
 #pragma unroll
@@ -746,10 +770,10 @@ __global__ void __launch_bounds__(kPaThreads, 1) k_pattn(const __grid_constant__
                         if (s >= n || !ok) break;
                         wait_stage();
                         if (!ok) break;
-                        score(s, h, 0);
+                        score(s, h, q0);
                         release();
                     }
-                if (n <= 2 && ok) commit(&ctl->qempty);
+                if (n <= 2 && ok) q_done();
                 for (int t = 0; t < n && ok; ++t) {
                     const bool more = t + 2 < n;
 #pragma unroll
@@ -761,11 +785,11 @@ __global__ void __launch_bounds__(kPaThreads, 1) k_pattn(const __grid_constant__
                         if (more) {
                             wait_stage();
                             if (!ok) break;
-                            score(t & 1, h, 0);
+                            score(t & 1, h, q0);
                             release();
                         }
                     }
-                    if (t + 3 == n && ok) commit(&ctl->qempty);
+                    if (t + 3 == n && ok) q_done();
                 }
             }
             tiles += n;
@@ -777,6 +801,7 @@ __global__ void __launch_bounds__(kPaThreads, 1) k_pattn(const __grid_constant__
         __syncwarp();
     } else if (warp == 10) {
         // ---------------- V rows that no row of the item may see become zero ----------------
+        const int vbox = min(ps, kPaKeys / 2);
         for (uint32_t r = 0;; ++r) {
             // no request may come for long; the TMA warp always posts the last one, and itself waits for 2 s at most
             bool there = false;
@@ -790,7 +815,7 @@ __global__ void __launch_bounds__(kPaThreads, 1) k_pattn(const __grid_constant__
             for (int q = lane >> 3; q < 64; q += 4)
                 if (q < f.z || q >= hi || !(f.w >> (16 + (q >> 4)) & 1))
                     for (int h = 0; h < NH; ++h)
-                        asm volatile("st.shared.v4.u32 [%0], {%1, %1, %1, %1};" ::"r"(kvs + f.x * STAGE + h * kSHalf + q * 128 + (lane & 7) * 16),
+                        asm volatile("st.shared.v4.u32 [%0], {%1, %1, %1, %1};" ::"r"(kvs + f.x * STAGE + (q / vbox * NH + h) * vbox * 128 + q % vbox * 128 + (lane & 7) * 16),
                                      "r"(0)
                                      : "memory");
             asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
@@ -1256,10 +1281,11 @@ int run_tc(const sd_attn_args& a, int dev, cudaStream_t st) {
         if (rc) return rc;
     }
     for (int i = 0; i < 2; ++i) {
-        const cuuint64_t dims[4] = {hd, (cuuint64_t)k.page_size, (cuuint64_t)k.n_kv_heads, (cuuint64_t)k.n_pages};
-        const cuuint64_t strides[3] = {(cuuint64_t)k.pos_stride * 2, (cuuint64_t)k.head_stride * 2, (cuuint64_t)k.page_stride * 2};
-        const cuuint32_t box[4] = {64, (cuuint32_t)std::min(k.page_size, kPaKeys / 2), 1, 1};
-        const int rc = encode(i ? &p.tv : &p.tk, bf, 4, i ? k.v : k.k, dims, strides, box);
+        const cuuint32_t rows = std::min(k.page_size, kPaKeys / 2), nh = k.head_dim / 64;
+        const cuuint64_t dims[5] = {64, (cuuint64_t)k.page_size, nh, (cuuint64_t)k.n_kv_heads, (cuuint64_t)k.n_pages};
+        const cuuint64_t strides[4] = {(cuuint64_t)k.pos_stride * 2, 128, (cuuint64_t)k.head_stride * 2, (cuuint64_t)k.page_stride * 2};
+        const cuuint32_t box[5] = {64, rows, i || rows == kPaKeys / 2 ? nh : 1, 1, 1};
+        const int rc = encode(i ? &p.tv : &p.tk, bf, 5, i ? k.v : k.k, dims, strides, box);
         if (rc) return rc;
     }
     const int pair = 2 * p.TPT;
