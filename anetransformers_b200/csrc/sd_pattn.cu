@@ -9,6 +9,7 @@
 #include <cuda_bf16.h>
 
 #include <algorithm>
+#include <cmath>
 #include <type_traits>
 
 #include "sd_common.cuh"
@@ -17,6 +18,18 @@
 
 using namespace sd;
 
+#ifndef PA_MIN
+#define PA_MIN 4
+#endif
+#ifndef PA_OV
+#define PA_OV 1.0
+#endif
+#ifndef PA_PMIN
+#define PA_PMIN 4
+#endif
+#ifndef PA_PR
+#define PA_PR 1
+#endif
 #ifndef PA_POLY
 #define PA_POLY 0
 #endif
@@ -181,9 +194,13 @@ __device__ __forceinline__ bool pa_inline(const PaArgs& p, int rows) { return p.
 __device__ __forceinline__ int pa_tiles(const PaArgs& p, int rows) {
     return rows <= p.TPT ? (rows > 0) : (rows + 2 * p.TPT - 1) / (2 * p.TPT);
 }
-__device__ __forceinline__ int pa_chunks(const PaArgs& p, int kv, bool inl) {
+// Chunks of a request's key tiles (the prefix's in front if it is inline) and tiles per chunk: as equal as they can be,
+// but with a window on a fixed grid, of which each item sees a part.
+__device__ __forceinline__ int pa_chunks(const PaArgs& p, int kv, bool inl, int* size) {
     const int t = (kv + kPaKeys - 1) / kPaKeys + (inl ? p.np : 0);
-    return max(1, (t + p.ct_own - 1) / p.ct_own);
+    const int n = max(1, (t + p.ct_own - 1) / p.ct_own);
+    *size = p.a.window > 0 ? p.ct_own : (t + n - 1) / n;
+    return n;
 }
 __device__ __forceinline__ int pa_request(const sd_attn_args& a, int tok) {
     int lo = 0, hi = a.n_req;
@@ -233,7 +250,8 @@ __device__ __forceinline__ bool pa_item(const PaArgs& p, const int* ustart, int 
     const int q = pa_q(a, b), kv = pa_kv(a, b), rows = pa_rows(a, b), nt = pa_tiles(p, rows);
     const bool inl = pa_inline(p, rows);
     const int c = local / nt, tile = nt - 1 - (local - c * nt);  // the tiles with most keys first
-    const int chunks = pa_chunks(p, kv, inl);
+    int size;
+    const int chunks = pa_chunks(p, kv, inl, &size);
     it.b = b;
     it.q0 = max(a.q_start[b], 0);
     it.rows = rows;
@@ -249,8 +267,8 @@ __device__ __forceinline__ bool pa_item(const PaArgs& p, const int* ustart, int 
     it.klo_p = W > 0 ? min(P, max(0, P + first + 1 - W)) : 0;
     int s0 = it.klo_o / kPaKeys + it.npt;
     if (inl && it.klo_p < P) s0 = it.klo_p / kPaKeys;
-    it.v0 = max(c * p.ct_own, s0);
-    const int end = min((c + 1) * p.ct_own, it.npt + (it.khi_o + kPaKeys - 1) / kPaKeys);
+    it.v0 = max(c * size, s0);
+    const int end = min((c + 1) * size, it.npt + (it.khi_o + kPaKeys - 1) / kPaKeys);
     it.n = last < 0 ? 0 : max(0, end - it.v0);
     it.split = p.cp + c;
     return true;
@@ -498,7 +516,8 @@ __global__ void __launch_bounds__(kPaThreads, 1) k_pattn(const __grid_constant__
         int sum = 0;
         bool bad = false;
         for (int b = b0; b < b1; ++b) {
-            const int rows = pa_rows(a, b), u = rows > 0 ? pa_tiles(p, rows) * pa_chunks(p, pa_kv(a, b), pa_inline(p, rows)) : 0;
+            int size;
+            const int rows = pa_rows(a, b), u = rows > 0 ? pa_tiles(p, rows) * pa_chunks(p, pa_kv(a, b), pa_inline(p, rows), &size) : 0;
             bad |= a.q_len[b] > a.max_q || a.q_len[b] < 0 || a.kv_len[b] > a.max_kv || a.kv_len[b] < 0 || a.q_start[b] < 0 ||
                    rows < pa_q(a, b);
             ustart[b] = u;
@@ -1140,7 +1159,8 @@ __global__ void __launch_bounds__(256) k_pattn_combine(const __grid_constant__ P
     if (t < 0 || t >= rows) return;
     const int kv = pa_kv(a, b);
     const bool inl = pa_inline(p, rows);
-    const int chunks = pa_chunks(p, kv, inl);
+    int size;
+    const int chunks = pa_chunks(p, kv, inl, &size);
     if (chunks == 1 && (a.prefix_len == 0 || inl)) return;  // written by its item
     const bool seeing = kv - pa_q(a, b) + t >= 0;
     const int s0 = inl ? p.cp : 0, s1 = seeing ? p.cp + chunks : s0;
@@ -1152,15 +1172,27 @@ __global__ void __launch_bounds__(256) k_pattn_combine(const __grid_constant__ P
     float L = 0.f, o[V];
 #pragma unroll
     for (int e = 0; e < V; ++e) o[e] = 0.f;
-    for (int s = s0; s < s1; ++s) {
-        const float2 ml = p.ml[s * ld + row];
-        if (ml.y == 0.f) continue;
-        const float f = ex2(ml.x - M);
+    for (int c = s0; c < s1; c += 32) {
+        // lane l: weight of split c + l (0 where it saw nothing, and its O is then not defined)
+        const float2 ml = c + lane < s1 ? p.ml[(c + lane) * ld + row] : make_float2(0.f, 0.f);
+        const float f = ml.y == 0.f ? 0.f : ex2(ml.x - M);
         L = fmaf(ml.y, f, L);
-        const float* acc = p.acc + (s * ld + row) * HD + lane * V;
+        for (int s = c; s < min(s1, c + 32); s += 8) {  // eight splits' O in flight
+            float acc[8][V];
 #pragma unroll
-        for (int e = 0; e < V; ++e) o[e] = fmaf(acc[e], f, o[e]);
+            for (int u = 0; u < 8; ++u) {
+                const float fu = __shfl_sync(0xffffffffu, f, (s - c + u) & 31);
+                const float* src = p.acc + ((s + u) * ld + row) * HD + lane * V;
+#pragma unroll
+                for (int e = 0; e < V; ++e) acc[u][e] = s + u < s1 && fu != 0.f ? src[e] * fu : 0.f;
+            }
+#pragma unroll
+            for (int u = 0; u < 8; ++u)
+#pragma unroll
+                for (int e = 0; e < V; ++e) o[e] += acc[u][e];
+        }
     }
+    L = warp_sum(L);
     const float inv = L > 0.f ? 1.f / L : (L == 0.f ? 0.f : L);
     uint32_t* dst = reinterpret_cast<uint32_t*>(static_cast<T*>(a.out) + (size_t)tok * a.out_ld + (size_t)head * a.out_head + lane * V);
 #pragma unroll
@@ -1204,19 +1236,33 @@ void pa_plan(const sd_attn_args& a, int sms, PaArgs* p) {
     const int n_kv = a.pool.n_kv_heads, pair = 2 * p->TPT;
     p->np = (a.prefix_len + kPaKeys - 1) / kPaKeys;
     const int own = (a.max_kv + kPaKeys - 1) / kPaKeys + (a.max_q > pair ? p->np : 0);
-    // own items: aim at four per SM, but not below 8 key tiles (an item costs about one tile to start and to join)
-    // over the tiles that an item can see through the window; if those fit one chunk, nothing is cut
     const long long units = (long long)n_kv * std::max<long long>(a.n_req, a.n_tokens / pair);
+    // tiles that an item can see through the window; if those fit one chunk, nothing is cut
     const int seen = a.window > 0 ? (int)std::min<long long>(own, ((long long)a.window + std::min(a.max_q, pair)) / kPaKeys + 2) : own;
-    long long ct = std::max<long long>(8, (units * seen + 4LL * sms - 1) / (4LL * sms));
-    p->ct_own = ct >= seen ? std::max(own, 1) : (int)ct;
-    // prefix items: the same over the tokens' row tiles
+    int ct = std::max(seen, 1);
+    if (a.max_q <= p->TPT) {
+        // few rows per item: a chunk costs about PA_OV tiles to start and to join, and the last one to end leaves the
+        // other SMs idle for up to its length: the sum is least at the square root of PA_OV times an SM's tiles
+        const double per_sm = (double)units * seen / sms;
+        ct = std::max(PA_MIN, (int)(std::sqrt(PA_OV * per_sm) + 0.5));
+    } else {
+        // many rows: whole rounds over the SMs; a cut costs about 3 tiles more (O of 256 rows in 32 bits, twice)
+        double best = 1e300;
+        for (int n = 1; n <= 8; ++n) {
+            const long long rounds = (units * n + sms - 1) / sms;
+            const double t = (double)rounds * ((seen + n - 1) / n + 1.5 + (n > 1 ? 3.0 : 0.0));
+            if (t < best * 0.97) best = t, ct = (seen + n - 1) / n;
+        }
+    }
+    p->ct_own = ct >= seen ? std::max(own, 1) : std::max(ct, 1);
+    // prefix items: one round over the SMs
     p->n_pt = p->np ? (a.n_tokens + pair - 1) / pair : 0;
     p->ct_pre = 1;
     p->cp = 0;
     if (p->np) {
-        ct = std::max<long long>(4, ((long long)n_kv * p->n_pt * p->np + 2LL * sms - 1) / (2LL * sms));
-        p->ct_pre = (int)std::min<long long>(p->np, ct);
+        const long long u = (long long)n_kv * p->n_pt;
+        const long long n = std::max<long long>(1, std::min<long long>((p->np + PA_PMIN - 1) / PA_PMIN, (long long)PA_PR * sms / u));
+        p->ct_pre = (int)((p->np + n - 1) / n);
         p->cp = (p->np + p->ct_pre - 1) / p->ct_pre;
     }
 }
