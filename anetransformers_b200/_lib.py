@@ -145,6 +145,7 @@ _SIGS = {
     "sd_tokenizer_apply_chat": (vp, [C.c_char_p]),
     "sd_free": (None, [vp]),
     "sd_batch_create": (i32, [vp, i32, i32, i32, vp]),
+    "sd_batch_create_shared": (i32, [vp, vp, i32, i32, i32, i32, vp]),
     "sd_batch_free": (None, [vp]),
     "sd_batch_stream": (vp, [vp]),
     "sd_batch_set_gemm": (i32, [vp, i32]),

@@ -21,6 +21,10 @@
 // emission are the single-stream kernels (sd_spec.cu), one CTA per stream.  Tokens of a stream beyond its
 // valid count (fewer drafts than T - 1, or a finished stream) are computed with stale activations and
 // dropped: they write no K/V and no output.
+//
+// A batch over a shared prefix (sd_batch_create_shared) keeps its K/V in pages: k_bpage_lens and the page plan
+// (sd_paged.cu) turn the streams' positions into block tables and slots once per forward, k_brope_kv writes through the
+// slots, and the attention over pages (sd_pattn.cu) with k_bq8 takes the place of k_battn_partial / k_battn_combine.
 #include <algorithm>
 #include <chrono>
 #include <cmath>
@@ -29,6 +33,7 @@
 
 #include "sd_dev.cuh"
 #include "sd_host.h"
+#include "sd_paged.h"
 #include "sd_spec.h"
 #include "specdec_b200.h"
 
@@ -147,6 +152,10 @@ struct BRopeArgs {
     const float* theta_inv;
     float q_scale;
     const DevCtrl* ctrl;
+    // paged batch: slot of each token in the layer's pool, fp16 q, and the positions in front of a stream's first
+    const int* slots;
+    __half* q16;
+    int pos0;
 };
 
 // RoPE of q and k (mistral/mistral_model.h:79-122, the matvec epilogue's arithmetic) and the fp16 K/V write
@@ -155,10 +164,17 @@ __global__ void __launch_bounds__(256) k_brope_kv(const BRopeArgs a) {
     int b, j;
     const int m = blockIdx.x;
     if (!token_valid(a.ctrl, m, a.T, &b, &j)) return;
-    const int tpos = a.ctrl[b].pos + j;
+    const int tpos = a.ctrl[b].pos + j + a.pos0;
     const int rows = a.q_rows + 2 * a.kv_rows;
     const float* src = a.qkv + (size_t)m * rows;
-    const size_t ring = (size_t)b * a.kv_stream + (size_t)(tpos % a.max_seq) * a.kv_rows;
+    size_t ring;
+    if (a.slots) {
+        const int slot = a.slots[m];
+        if (slot < 0) return;  // no page for it: the plan has counted it as missing
+        ring = (size_t)slot * a.kv_rows;
+    } else {
+        ring = (size_t)b * a.kv_stream + (size_t)(tpos % a.max_seq) * a.kv_rows;
+    }
     for (int pr = threadIdx.x; pr < rows / 2; pr += blockDim.x) {
         const int gr = 2 * pr;
         float ve = 0.f, vo = 0.f;
@@ -174,7 +190,9 @@ __global__ void __launch_bounds__(256) k_brope_kv(const BRopeArgs a) {
             sincosf(ang, &sn, &cs);
             const float e2 = fmaf(-vo, sn, ve * cs);
             const float o2 = fmaf(ve, sn, vo * cs);
-            if (gr < a.q_rows) {
+            if (gr < a.q_rows && a.q16) {
+                *reinterpret_cast<__half2*>(a.q16 + (size_t)m * a.q_rows + gr) = __halves2half2(__float2half_rn(e2), __float2half_rn(o2));
+            } else if (gr < a.q_rows) {
                 *reinterpret_cast<float2*>(a.q + (size_t)m * a.q_rows + gr) = make_float2(e2 * a.q_scale, o2 * a.q_scale);
             } else {
                 *reinterpret_cast<__half2*>(a.k + ring + (gr - a.q_rows)) = __halves2half2(__float2half_rn(e2), __float2half_rn(o2));
@@ -445,6 +463,32 @@ __global__ void __launch_bounds__(kAttnThreads, 2) k_battn_partial(const BAttnAr
     cp_async_wait_all();
 }
 
+// Q8_0 of one token's head output (lane = 4 dims) in the o-proj image.
+__device__ __forceinline__ void store_q8_head(const WImg& img, int tok, int h, int lane, const float (&o)[4]) {
+    // Q8_0 blocks: dims [32*bk, 32*bk+32) are lanes 8*bk..8*bk+7 (4 values each), as attn_combine_row
+    float am = fmaxf(fmaxf(fabsf(o[0]), fabsf(o[1])), fmaxf(fabsf(o[2]), fabsf(o[3])));
+#pragma unroll
+    for (int off = 4; off > 0; off >>= 1) am = fmaxf(am, __shfl_xor_sync(0xffffffffu, am, off));
+    const float d = __fdiv_rn(am, 127.0f);
+    int q[4] = {0, 0, 0, 0};
+    if (am != 0.0f) {
+        const float id = __fdiv_rn(1.0f, d);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            const int r = __float2int_rn(__fmul_rn(o[e], id));
+            q[e] = r > 127 ? 127 : (r < -128 ? -128 : r);
+        }
+    }
+    int qsum = q[0] + q[1] + q[2] + q[3];
+#pragma unroll
+    for (int off = 4; off > 0; off >>= 1) qsum += __shfl_xor_sync(0xffffffffu, qsum, off);
+    const uint32_t packed = (uint32_t)(q[0] & 0xFF) | ((uint32_t)(q[1] & 0xFF) << 8) | ((uint32_t)(q[2] & 0xFF) << 16) |
+                            ((uint32_t)(q[3] & 0xFF) << 24);
+    const int blk = h * (kHD / 32) + (lane >> 3);
+    wimg_put_word(img, tok, blk, lane & 7, packed);
+    if ((lane & 7) == 0) wimg_put_meta(img, tok, blk, d, qsum);
+}
+
 // Merge of the chunk partials of one (token, head) row and its Q8_0 quantisation into the o-proj image: one
 // warp per row, eight rows per CTA.  Lane l holds the (max, sum) pair of chunk c0 + l; every chunk's max and sum
 // and the first eight chunks' 128-dim partials (lane = 4 dims) are loaded in one round trip.  The chunks are
@@ -503,28 +547,30 @@ __global__ void __launch_bounds__(kBCombWarps * 32) k_battn_combine(const BAttnA
     const float inv = 1.0f / L;
 #pragma unroll
     for (int e = 0; e < 4; ++e) o[e] *= inv;
-    // Q8_0 blocks: dims [32*bk, 32*bk+32) are lanes 8*bk..8*bk+7 (4 values each), as attn_combine_row
-    float am = fmaxf(fmaxf(fabsf(o[0]), fabsf(o[1])), fmaxf(fabsf(o[2]), fabsf(o[3])));
-#pragma unroll
-    for (int off = 4; off > 0; off >>= 1) am = fmaxf(am, __shfl_xor_sync(0xffffffffu, am, off));
-    const float d = __fdiv_rn(am, 127.0f);
-    int q[4] = {0, 0, 0, 0};
-    if (am != 0.0f) {
-        const float id = __fdiv_rn(1.0f, d);
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-            const int r = __float2int_rn(__fmul_rn(o[e], id));
-            q[e] = r > 127 ? 127 : (r < -128 ? -128 : r);
-        }
-    }
-    int qsum = q[0] + q[1] + q[2] + q[3];
-#pragma unroll
-    for (int off = 4; off > 0; off >>= 1) qsum += __shfl_xor_sync(0xffffffffu, qsum, off);
-    const uint32_t packed = (uint32_t)(q[0] & 0xFF) | ((uint32_t)(q[1] & 0xFF) << 8) | ((uint32_t)(q[2] & 0xFF) << 16) |
-                            ((uint32_t)(q[3] & 0xFF) << 24);
-    const int blk = h * (kHD / 32) + (lane >> 3);
-    wimg_put_word(a.wimg, a.tok0 + s, blk, lane & 7, packed);
-    if ((lane & 7) == 0) wimg_put_meta(a.wimg, a.tok0 + s, blk, d, qsum);
+    store_q8_head(a.wimg, a.tok0 + s, h, lane, o);
+}
+
+// Paged batch: fp16 head outputs -> Q8_0 in the o-proj image, one warp per (token, head).
+__global__ void __launch_bounds__(kBCombWarps * 32) k_bq8(const __half* x, WImg img, int n_heads, int M, int T, const DevCtrl* ctrl) {
+    const int row = blockIdx.x * kBCombWarps + (threadIdx.x >> 5), lane = threadIdx.x & 31;
+    if (row >= M * n_heads) return;
+    const int m = row / n_heads, h = row - m * n_heads;
+    int b, s;
+    if (!token_valid(ctrl, m, T, &b, &s)) return;
+    const __half2* src = reinterpret_cast<const __half2*>(x + ((size_t)m * n_heads + h) * kHD + lane * 4);
+    const float2 lo = __half22float2(src[0]), hi = __half22float2(src[1]);
+    const float o[4] = {lo.x, lo.y, hi.x, hi.y};
+    store_q8_head(img, m, h, lane, o);
+}
+
+// Lengths of a forward for the page plan: stream b has pos + nv positions behind the prefix, nv of them new (a finished
+// stream keeps its positions); row n is the prefix itself.
+__global__ void k_bpage_lens(const DevCtrl* ctrl, int n, int T, int prefix, int* kv_len, int* q_len) {
+    const int b = blockIdx.x * blockDim.x + threadIdx.x;
+    if (b > n) return;
+    const int nv = b == n || ctrl[b].done ? 0 : min(ctrl[b].n_valid, T);
+    kv_len[b] = b == n ? prefix : ctrl[b].pos + nv;
+    q_len[b] = nv;
 }
 
 // Control blocks of a forward of T tokens per stream: tokens[b * stride + col0 + j], position pos[b] (or col0).
@@ -663,6 +709,15 @@ struct sd_batch {
     int* ndone = nullptr;     // [2]: streams done, most tokens a live stream still has to generate
     int* ndone_h = nullptr;   // pinned copy
     int gemm_mode = SD_BATCH_GEMM_AUTO;
+    // paged batch: positions in front of every stream's first, pages of kPage positions ([layer][n_pages][kPage][kv_rows]
+    // in kc / vc), block tables of the streams and (row B) the prefix
+    int prefix = 0;
+    bool paged = false, filling = false;  // filling: the forward computes the prefix itself (row B), in slices
+    sd_pages pages{};
+    int *kv_len = nullptr, *q_len = nullptr, *q_start = nullptr, *slots = nullptr;
+    __half *q16 = nullptr, *o16 = nullptr;  // [M_max][q_rows]
+    uint8_t* attn_ws = nullptr;
+    size_t attn_ws_bytes = 0;
     bool shared_ring = false;  // kc / vc and st belong to the context (GEMM prefill of a single stream)
     BPlans plans[SD_BATCH_MAX_WIDTH + 1];
     cudaGraphExec_t fwd_graph[SD_BATCH_MAX_WIDTH + 1][2] = {};
@@ -672,6 +727,8 @@ struct sd_batch {
 };
 
 namespace {
+
+constexpr int kPage = 64;  // positions per page of a paged batch: a ring stage of the attention is one box
 
 int ck(cudaError_t e, const char* what) { return e == cudaSuccess ? SD_OK : cuda_fail(e, what); }
 
@@ -734,6 +791,72 @@ int run_wgemm(sd_batch* b, int epi, WgPlan p, const uint8_t* w, const uint8_t* a
     return SD_OK;
 }
 
+// Attention of layer l over the streams' rings, head outputs as Q8_0 in img.
+int ring_attention(sd_batch* b, int T, int l, WImg img) {
+    const ModelView& m = b->m;
+    const int M = b->B * T;
+    BAttnArgs ba{};
+    ba.a.q = b->q;
+    ba.a.q_ld = m.q_rows;
+    ba.a.k = b->kc + (size_t)l * b->kv_layer;
+    ba.a.v = b->vc + (size_t)l * b->kv_layer;
+    ba.a.kv_ld = m.kv_rows;
+    ba.a.n_heads = m.n_heads;
+    ba.a.n_kvh = m.n_kv;
+    ba.a.S = T;
+    ba.a.max_seq = b->max_seq;
+    ba.a.chunk = b->chunk;
+    ba.a.max_chunks = b->max_chunks;
+    ba.a.part_ml = b->part_ml;
+    ba.a.part_acc = b->part_acc;
+    ba.a.wimg = img;
+    ba.kv_stream = b->kv_stream;
+    ba.T = T;
+    ba.ctrl = b->ctrl;
+    ba.n_streams = b->B;
+    k_battn_partial<<<std::min(2 * b->sms, b->B * b->max_chunks * m.n_kv), kAttnThreads, battn_smem_bytes(), b->st>>>(ba);
+    CK(cudaGetLastError(), "attention");
+    k_battn_combine<<<(M * m.n_heads + kBCombWarps - 1) / kBCombWarps, kBCombWarps * 32, 0, b->st>>>(ba);
+    CK(cudaGetLastError(), "combine");
+    return SD_OK;
+}
+
+// Attention of layer l over the pages, head outputs in o16: T tokens of every stream behind the prefix, or (filling) the
+// prefix's own next tokens.
+sd_attn_args paged_args(const sd_batch* b, int T, int l) {
+    const ModelView& m = b->m;
+    sd_attn_args a{};
+    a.pool = sd_kv_pool{b->kc + (size_t)l * b->kv_layer, b->vc + (size_t)l * b->kv_layer, (int64_t)kPage * m.kv_rows, m.kv_rows, m.hd,
+                        b->pages.n_pages, kPage, m.n_kv, m.hd, SD_F16};
+    a.q = b->q16;
+    a.out = b->o16;
+    a.q_ld = a.out_ld = m.q_rows;
+    a.q_head = a.out_head = m.hd;
+    const int32_t* prefix = b->pages.table + (size_t)b->B * b->pages.table_ld;
+    const int row = b->filling ? b->B : 0;
+    a.table = b->pages.table + (size_t)row * b->pages.table_ld;
+    a.kv_len = b->kv_len + row;
+    a.q_start = b->q_start + row;
+    a.q_len = b->q_len + row;
+    a.n_req = b->filling ? 1 : b->B;
+    a.n_tokens = b->B * T;
+    a.n_heads = m.n_heads;
+    a.table_ld = b->pages.table_ld;
+    a.max_q = b->filling ? b->B * T : T;
+    a.max_kv = b->filling ? b->prefix : b->max_seq;
+    a.prefix_table = b->filling ? nullptr : prefix;
+    a.prefix_len = b->filling ? 0 : b->prefix;
+    a.scale = 1.0f / sqrtf((float)m.hd);
+    a.workspace = b->attn_ws;
+    a.workspace_bytes = b->attn_ws_bytes;
+    return a;
+}
+
+int paged_attention(sd_batch* b, int T, int l) {
+    const sd_attn_args a = paged_args(b, T, l);
+    return launch_paged_attention(&a, b->dev, b->m.err, b->st);
+}
+
 // One forward of T tokens per stream (positions and token ids from the control blocks).
 int enqueue_bforward(sd_batch* b, int T, bool logits) {
     const ModelView& m = b->m;
@@ -753,6 +876,16 @@ int enqueue_bforward(sd_batch* b, int T, bool logits) {
     na.w = m.rms_att[0];
     k_bnorm<0><<<M, kBNormThreads, 0, b->st>>>(na);
     CK(cudaGetLastError(), "embed");
+    if (b->paged) {
+        if (!b->filling) {
+            k_bpage_lens<<<b->B / 128 + 1, 128, 0, b->st>>>(b->ctrl, b->B, T, b->prefix, b->kv_len, b->q_len);
+            CK(cudaGetLastError(), "lengths");
+        }
+        // the prefix's slices are one request's tokens in a row, a stream's are T apart
+        const int rc = launch_pages_plan(&b->pages, b->kv_len, b->q_len, b->filling ? 0 : T, 0, M, b->q_start, b->slots, nullptr,
+                                         nullptr, m.err, b->st);
+        if (rc) return rc;
+    }
     for (int l = 0; l < m.n_layers; ++l) {
         int rc;
         // QKV
@@ -778,32 +911,21 @@ int enqueue_bforward(sd_batch* b, int T, bool logits) {
         ra.theta_inv = m.theta_inv;
         ra.q_scale = 1.0f / sqrtf((float)m.hd);
         ra.ctrl = b->ctrl;
+        if (b->paged) {
+            ra.slots = b->slots;
+            ra.q16 = b->q16;
+            ra.pos0 = b->filling ? 0 : b->prefix;
+        }
         k_brope_kv<<<M, 256, 0, b->st>>>(ra);
         CK(cudaGetLastError(), "rope");
-        // attention
-        BAttnArgs ba{};
-        ba.a.q = b->q;
-        ba.a.q_ld = m.q_rows;
-        ba.a.k = ra.k;
-        ba.a.v = ra.v;
-        ba.a.kv_ld = m.kv_rows;
-        ba.a.n_heads = m.n_heads;
-        ba.a.n_kvh = m.n_kv;
-        ba.a.S = T;
-        ba.a.max_seq = b->max_seq;
-        ba.a.chunk = b->chunk;
-        ba.a.max_chunks = b->max_chunks;
-        ba.a.part_ml = b->part_ml;
-        ba.a.part_acc = b->part_acc;
-        ba.a.wimg = WImg{b->img_attn, NT, tcimg};
-        ba.kv_stream = b->kv_stream;
-        ba.T = T;
-        ba.ctrl = b->ctrl;
-        ba.n_streams = b->B;
-        k_battn_partial<<<std::min(2 * b->sms, b->B * b->max_chunks * m.n_kv), kAttnThreads, battn_smem_bytes(), b->st>>>(ba);
-        CK(cudaGetLastError(), "attention");
-        k_battn_combine<<<(M * m.n_heads + kBCombWarps - 1) / kBCombWarps, kBCombWarps * 32, 0, b->st>>>(ba);
-        CK(cudaGetLastError(), "combine");
+        if (b->paged) {
+            if ((rc = paged_attention(b, T, l))) return rc;
+            k_bq8<<<(M * m.n_heads + kBCombWarps - 1) / kBCombWarps, kBCombWarps * 32, 0, b->st>>>(
+                b->o16, WImg{b->img_attn, NT, tcimg}, m.n_heads, M, T, b->ctrl);
+            CK(cudaGetLastError(), "head outputs");
+        } else if ((rc = ring_attention(b, T, l, WImg{b->img_attn, NT, tcimg}))) {
+            return rc;
+        }
         // o-proj, residual + norm
         WgPlan po = P.wo;
         po.a.out = b->y;
@@ -1030,6 +1152,9 @@ void sd_batch_free(sd_batch* b) {
     cudaFree(b->x); cudaFree(b->y); cudaFree(b->qkv); cudaFree(b->q);
     cudaFree(b->img_x); cudaFree(b->img_attn); cudaFree(b->img_h); cudaFree(b->part_ml); cudaFree(b->part_acc);
     cudaFree(b->logits); cudaFree(b->argmax); cudaFree(b->probs); cudaFree(b->ctrl); cudaFree(b->tok);
+    cudaFree(b->pages.table); cudaFree(b->pages.held); cudaFree(b->pages.free_pages); cudaFree(b->pages.n_free);
+    cudaFree(b->kv_len); cudaFree(b->q_len); cudaFree(b->q_start); cudaFree(b->slots);
+    cudaFree(b->q16); cudaFree(b->o16); cudaFree(b->attn_ws);
     cudaFree(b->pos_dev); cudaFree(b->gs); cudaFree(b->g_out); cudaFree(b->g_hist); cudaFree(b->ndone);
     if (b->gs_h) cudaFreeHost(b->gs_h);
     if (b->ndone_h) cudaFreeHost(b->ndone_h);
@@ -1068,7 +1193,8 @@ struct SharedRing {
     cudaStream_t st;
 };
 
-int batch_create(sd_ctx* ctx, int n_streams, int max_seq, int max_width, const SharedRing* shared, sd_batch** out) {
+// n_prefix > 0: a paged batch behind a prefix of that many positions (filled by the caller).
+int batch_create(sd_ctx* ctx, int n_streams, int max_seq, int max_width, const SharedRing* shared, int n_prefix, sd_batch** out) {
     *out = nullptr;
     sd_batch* b = new sd_batch();
     int rc = sd_ctx_model_view(ctx, &b->m);
@@ -1107,6 +1233,28 @@ int batch_create(sd_ctx* ctx, int n_streams, int max_seq, int max_width, const S
     b->kv_stream = shared ? 0 : (size_t)max_seq * m.kv_rows;
     b->kv_layer = shared ? (size_t)max_seq * m.kv_rows : (size_t)n_streams * b->kv_stream;
     const size_t M = b->M_max;
+    if (n_prefix > 0) {
+        b->paged = true;
+        b->prefix = n_prefix;
+        b->max_chunks = 1;  // no ring attention: one partial row each
+        const long long per = (max_seq + kPage - 1) / kPage, pre = (n_prefix + kPage - 1) / kPage, n = pre + per * n_streams;
+        if (n * kPage > INT32_MAX || n_streams + 1 > SD_PAGES_MAX_REQ)
+            return bail(fail(SD_ERR_UNSUPPORTED, "%d streams of %d positions behind a prefix of %d", n_streams, max_seq, n_prefix));
+        b->kv_layer = (size_t)n * kPage * m.kv_rows;
+        sd_pages& g = b->pages;
+        g.n_req = n_streams + 1;
+        g.table_ld = (int)std::max(per, pre);
+        g.n_pages = (int)n;
+        g.page_size = kPage;
+        if ((rc = dalloc(&g.table, (size_t)g.n_req * g.table_ld)) || (rc = dalloc(&g.held, g.n_req)) ||
+            (rc = dalloc(&g.free_pages, g.n_pages)) || (rc = dalloc(&g.n_free, 1)) || (rc = dalloc(&b->kv_len, g.n_req)) ||
+            (rc = dalloc(&b->q_len, g.n_req)) || (rc = dalloc(&b->q_start, g.n_req)) || (rc = dalloc(&b->slots, M)) ||
+            (rc = dalloc(&b->q16, M * m.q_rows)) || (rc = dalloc(&b->o16, M * m.q_rows)))
+            return bail(rc);
+        if ((rc = sd_pages_reset_dev(&g, b->st))) return bail(rc);
+        cudaMemsetAsync(b->o16, 0, M * m.q_rows * sizeof(__half), b->st);
+        cudaMemsetAsync(b->q16, 0, M * m.q_rows * sizeof(__half), b->st);
+    }
     const size_t parts = (size_t)M * m.n_heads * b->max_chunks;
     if ((!shared && ((rc = dalloc(&b->kc, (size_t)m.n_layers * b->kv_layer)) ||
                      (rc = dalloc(&b->vc, (size_t)m.n_layers * b->kv_layer)))) ||
@@ -1119,6 +1267,17 @@ int batch_create(sd_ctx* ctx, int n_streams, int max_seq, int max_width, const S
         (rc = dalloc(&b->ctrl, (size_t)n_streams)) || (rc = dalloc(&b->pos_dev, (size_t)n_streams)) ||
         (rc = dalloc(&b->gs, (size_t)n_streams)) || (rc = dalloc(&b->ndone, 2)))
         return bail(rc);
+    if (b->paged) {
+        // the largest workspace of any forward
+        for (int f = 0; f < 2; ++f)
+            for (int T = 1; T <= max_width; ++T) {
+                b->filling = f != 0;
+                const sd_attn_args a = paged_args(b, T, 0);
+                b->attn_ws_bytes = std::max(b->attn_ws_bytes, sd_attention_workspace(&a));
+            }
+        b->filling = false;
+        if (b->attn_ws_bytes && (rc = dalloc(&b->attn_ws, b->attn_ws_bytes))) return bail(rc);
+    }
     // weights in the wide GEMM layout (the context keeps its tile16x4 copies for the single-stream path)
     auto wide = [&](const uint8_t* tiles, int rows, int cols, uint8_t** out_w) {
         int r = dalloc(out_w, wide_bytes(rows, cols));
@@ -1161,7 +1320,7 @@ int sd_batch_create(sd_ctx* ctx, int n_streams, int max_seq, int max_width, sd_b
     clear_error();
     if (!ctx || !out || n_streams < 1 || max_seq < 16 || max_width < 1 || max_width > SD_BATCH_MAX_WIDTH)
         return fail(SD_ERR_INVALID, "sd_batch_create: bad arguments");
-    return batch_create(ctx, n_streams, max_seq, max_width, nullptr, out);
+    return batch_create(ctx, n_streams, max_seq, max_width, nullptr, 0, out);
 }
 
 }  // extern "C"
@@ -1171,7 +1330,7 @@ namespace sd {
 int batch_create_prefill(sd_ctx* ctx, int n_slices, int width, void* kc, void* vc, int max_seq, cudaStream_t st,
                          sd_batch** out) {
     const SharedRing sr{reinterpret_cast<__half*>(kc), reinterpret_cast<__half*>(vc), st};
-    return batch_create(ctx, n_slices, max_seq, width, &sr, out);
+    return batch_create(ctx, n_slices, max_seq, width, &sr, 0, out);
 }
 
 // Chunks of n_slices x width prompt tokens; slice v of a chunk starting at prompt index i takes tokens
@@ -1201,7 +1360,58 @@ int batch_prefill_ring(sd_batch* b, const int32_t* tokens, int n, int start_pos)
 
 }  // namespace sd
 
+namespace {
+
+// K/V of the prefix into the pages of row B: chunks of all the forward's tokens, cut into slices of max_width tokens as
+// batch_prefill_ring does.
+int fill_prefix(sd_batch* b, const int32_t* tokens) {
+    const int W = b->W, chunk = b->B * W, n = b->prefix;
+    std::vector<DevCtrl> hc(b->B);
+    std::vector<int32_t> kv(b->B + 1, 0), q(b->B + 1, 0);
+    b->filling = true;
+    int rc = SD_OK;
+    for (int i = 0; i < n && !rc; i += chunk) {
+        for (int v = 0; v < b->B; ++v) {
+            DevCtrl& c = hc[v];
+            memset(&c, 0, sizeof(c));
+            const int first = i + v * W, nv = std::max(0, std::min(W, n - first));
+            c.pos = first;
+            c.n_valid = nv;
+            c.done = nv == 0;
+            for (int j = 0; j < nv; ++j) c.tokens[j] = tokens[first + j];
+        }
+        q[b->B] = std::min(chunk, n - i);
+        kv[b->B] = i + q[b->B];
+        // from pageable memory: each call returns once the host array has been read
+        rc = ck(cudaMemcpyAsync(b->ctrl, hc.data(), sizeof(DevCtrl) * b->B, cudaMemcpyHostToDevice, b->st), "prefix ctrl");
+        if (!rc) rc = ck(cudaMemcpyAsync(b->kv_len, kv.data(), 4 * kv.size(), cudaMemcpyHostToDevice, b->st), "prefix lengths");
+        if (!rc) rc = ck(cudaMemcpyAsync(b->q_len, q.data(), 4 * q.size(), cudaMemcpyHostToDevice, b->st), "prefix lengths");
+        if (!rc) rc = enqueue_bforward(b, W, false);
+    }
+    b->filling = false;
+    if (!rc) rc = ck(cudaMemsetAsync(b->ctrl, 0, sizeof(DevCtrl) * b->B, b->st), "ctrl");
+    return rc ? rc : finish(b);
+}
+
+}  // namespace
+
 extern "C" {
+
+int sd_batch_create_shared(sd_ctx* ctx, const int32_t* prefix, int n_prefix, int n_streams, int max_seq, int max_width,
+                           sd_batch** out) {
+    clear_error();
+    if (!ctx || !out || !prefix || n_prefix < 1 || n_streams < 1 || max_seq < 16 || max_width < 1 || max_width > SD_BATCH_MAX_WIDTH ||
+        (int64_t)n_prefix + max_seq > INT32_MAX / 2)
+        return fail(SD_ERR_INVALID, "sd_batch_create_shared: bad arguments");
+    int rc = batch_create(ctx, n_streams, max_seq, max_width, nullptr, n_prefix, out);
+    if (rc) return rc;
+    sd_batch* b = *out;
+    if ((rc = check_host_tokens(b, prefix, (size_t)n_prefix)) || (rc = fill_prefix(b, prefix))) {
+        sd_batch_free(b);
+        *out = nullptr;
+    }
+    return rc;
+}
 
 int sd_batch_forward(sd_batch* b, const int32_t* tokens, int T, const int32_t* pos, float* logits) {
     clear_error();

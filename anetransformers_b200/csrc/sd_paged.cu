@@ -311,6 +311,34 @@ void launch_append(const AppendArgs& a, bool vec, cudaStream_t st) {
 }
 
 }  // namespace
+
+int launch_pages_plan(const sd_pages* p, const int32_t* kv_len, const int32_t* q_len, int q_stride, int pos0, int n_tokens,
+                      int32_t* q_start, int32_t* slots, int32_t* positions, int32_t* missing, int* err, cudaStream_t st) {
+    PlanArgs a{p->table, p->held, p->free_pages, p->n_free, p->n_req, p->table_ld, p->n_pages, p->page_size,
+               kv_len, q_len, q_stride, pos0, n_tokens, q_start, slots, positions, missing, err};
+    const size_t smem = ((size_t)4 * p->n_req + 3) * sizeof(int);
+    cudaError_t e = cudaSuccess;
+    if (smem > 48 * 1024 - 1024)
+        e = cudaFuncSetAttribute(k_pages_plan, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+    if (e != cudaSuccess) return cuda_fail(e, "pages plan");
+    const int items = std::max(n_tokens, p->n_req);
+    int ctas = 1;
+    while (ctas < 8 && ctas * kPlanThreads < items) ctas *= 2;
+    cudaLaunchConfig_t cfg{};
+    cfg.gridDim = dim3(ctas);
+    cfg.blockDim = dim3(kPlanThreads);
+    cfg.dynamicSmemBytes = smem;
+    cfg.stream = st;
+    cudaLaunchAttribute at{};
+    at.id = cudaLaunchAttributeClusterDimension;
+    at.val.clusterDim.x = ctas;
+    at.val.clusterDim.y = at.val.clusterDim.z = 1;
+    cfg.attrs = &at;
+    cfg.numAttrs = 1;
+    e = cudaLaunchKernelEx(&cfg, k_pages_plan, (const PlanArgs)a);
+    return e == cudaSuccess ? SD_OK : cuda_fail(e, "pages plan");
+}
+
 }  // namespace sd
 
 extern "C" {
@@ -334,29 +362,8 @@ int sd_pages_plan_dev(const sd_pages* p, const int32_t* kv_len, const int32_t* q
     if ((int64_t)p->n_req * q_stride > INT32_MAX || (int64_t)pos0 + (int64_t)p->table_ld * p->page_size > INT32_MAX)
         return fail(SD_ERR_INVALID, "sd_pages_plan_dev: q_stride %d or pos0 %d too large", q_stride, pos0);
     if ((rc = paged_device(p->table, "sd_pages_plan_dev", &dev))) return rc;
-    PlanArgs a{p->table, p->held, p->free_pages, p->n_free, p->n_req, p->table_ld, p->n_pages, p->page_size,
-               kv_len, q_len, q_stride, pos0, n_tokens, q_start, slots, positions, missing, device_error_word(dev)};
-    const size_t smem = ((size_t)4 * p->n_req + 3) * sizeof(int);
-    cudaError_t e = cudaSuccess;
-    if (smem > 48 * 1024 - 1024)
-        e = cudaFuncSetAttribute(k_pages_plan, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
-    if (e != cudaSuccess) return cuda_fail(e, "pages plan");
-    const int items = std::max(n_tokens, p->n_req);
-    int ctas = 1;
-    while (ctas < 8 && ctas * kPlanThreads < items) ctas *= 2;
-    cudaLaunchConfig_t cfg{};
-    cfg.gridDim = dim3(ctas);
-    cfg.blockDim = dim3(kPlanThreads);
-    cfg.dynamicSmemBytes = smem;
-    cfg.stream = (cudaStream_t)stream;
-    cudaLaunchAttribute at{};
-    at.id = cudaLaunchAttributeClusterDimension;
-    at.val.clusterDim.x = ctas;
-    at.val.clusterDim.y = at.val.clusterDim.z = 1;
-    cfg.attrs = &at;
-    cfg.numAttrs = 1;
-    e = cudaLaunchKernelEx(&cfg, k_pages_plan, (const PlanArgs)a);
-    return e == cudaSuccess ? SD_OK : cuda_fail(e, "pages plan");
+    return launch_pages_plan(p, kv_len, q_len, q_stride, pos0, n_tokens, q_start, slots, positions, missing, device_error_word(dev),
+                             (cudaStream_t)stream);
 }
 
 int sd_kv_append_dev(const sd_kv_pool* pool, const void* k, const void* v, int src_dtype, int64_t k_ld, int64_t v_ld,

@@ -9,6 +9,7 @@
 #include <cuda_bf16.h>
 
 #include <algorithm>
+#include <atomic>
 #include <cmath>
 #include <type_traits>
 
@@ -1293,10 +1294,15 @@ int encode(CUtensorMap* m, bool bf16, int rank, const void* base, const cuuint64
 static_assert(pa_smem<128>(SD_PAGES_MAX_REQ) <= 232448, "the largest batch fits the shared memory");
 
 template <class T, int HD, bool MOD>
-int launch_tc(const PaArgs& p, int grid, cudaStream_t st) {
+int launch_tc(const PaArgs& p, int grid, int dev, cudaStream_t st) {
     const size_t smem = pa_smem<HD>(p.a.n_req);
-    cudaError_t e = cudaFuncSetAttribute(k_pattn<T, HD, MOD>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
-    if (e != cudaSuccess) return cuda_fail(e, "attention attributes");
+    static std::atomic<bool> ready[64];  // per device: the largest batch's shared memory is allowed
+    cudaError_t e = cudaSuccess;
+    if (dev < 0 || dev >= 64 || !ready[dev].load(std::memory_order_acquire)) {
+        e = cudaFuncSetAttribute(k_pattn<T, HD, MOD>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)pa_smem<HD>(SD_PAGES_MAX_REQ));
+        if (e != cudaSuccess) return cuda_fail(e, "attention attributes");
+        if (dev >= 0 && dev < 64) ready[dev].store(true, std::memory_order_release);
+    }
     k_pattn<T, HD, MOD><<<grid, kPaThreads, smem, st>>>(p);
     if ((e = cudaGetLastError()) != cudaSuccess) return cuda_fail(e, "attention");
     if (pa_splits(p) > 0) {
@@ -1306,7 +1312,7 @@ int launch_tc(const PaArgs& p, int grid, cudaStream_t st) {
     return SD_OK;
 }
 
-int run_tc(const sd_attn_args& a, int dev, cudaStream_t st) {
+int run_tc(const sd_attn_args& a, int dev, int* err, cudaStream_t st) {
     PaArgs p{};
     pa_plan(a, device_sm_count(dev), &p);
     const size_t need = pa_workspace(p);
@@ -1315,7 +1321,7 @@ int run_tc(const sd_attn_args& a, int dev, cudaStream_t st) {
     const size_t rows = (size_t)pa_splits(p) * a.n_tokens * a.n_heads;
     p.acc = static_cast<float*>(a.workspace);
     p.ml = reinterpret_cast<float2*>(p.acc + rows * a.pool.head_dim);
-    p.err = device_error_word(dev);
+    p.err = err;
     const sd_kv_pool& k = a.pool;
     const bool bf = k.dtype == SD_BF16;
     const cuuint64_t hd = k.head_dim;
@@ -1342,11 +1348,11 @@ int run_tc(const sd_attn_args& a, int dev, cudaStream_t st) {
     const int grid = (int)items;
     const bool mod = a.softcap > 0.f || a.alibi || !(a.scale > 0.f);
     if (bf) {
-        if (k.head_dim == 128) return mod ? launch_tc<__nv_bfloat16, 128, true>(p, grid, st) : launch_tc<__nv_bfloat16, 128, false>(p, grid, st);
-        return mod ? launch_tc<__nv_bfloat16, 64, true>(p, grid, st) : launch_tc<__nv_bfloat16, 64, false>(p, grid, st);
+        if (k.head_dim == 128) return mod ? launch_tc<__nv_bfloat16, 128, true>(p, grid, dev, st) : launch_tc<__nv_bfloat16, 128, false>(p, grid, dev, st);
+        return mod ? launch_tc<__nv_bfloat16, 64, true>(p, grid, dev, st) : launch_tc<__nv_bfloat16, 64, false>(p, grid, dev, st);
     }
-    if (k.head_dim == 128) return mod ? launch_tc<__half, 128, true>(p, grid, st) : launch_tc<__half, 128, false>(p, grid, st);
-    return mod ? launch_tc<__half, 64, true>(p, grid, st) : launch_tc<__half, 64, false>(p, grid, st);
+    if (k.head_dim == 128) return mod ? launch_tc<__half, 128, true>(p, grid, dev, st) : launch_tc<__half, 128, false>(p, grid, dev, st);
+    return mod ? launch_tc<__half, 64, true>(p, grid, dev, st) : launch_tc<__half, 64, false>(p, grid, dev, st);
 }
 
 int check_attention(const sd_attn_args* a) {
@@ -1375,6 +1381,20 @@ int check_attention(const sd_attn_args* a) {
 }
 
 }  // namespace
+
+int launch_paged_attention(const sd_attn_args* a, int dev, int* err, cudaStream_t st) {
+    if (tc_able(*a)) return run_tc(*a, dev, err, st);
+    const long long rows = (long long)a->n_tokens * a->n_heads;
+    if ((rows + 3) / 4 > INT32_MAX) return fail(SD_ERR_INVALID, "sd_attention_dev: too many rows");
+    const int grid = (int)((rows + 3) / 4);
+    if (a->pool.dtype == SD_F16)
+        k_pattn_general<__half><<<grid, 128, 0, st>>>(*a, err);
+    else
+        k_pattn_general<__nv_bfloat16><<<grid, 128, 0, st>>>(*a, err);
+    const cudaError_t e = cudaGetLastError();
+    return e == cudaSuccess ? SD_OK : cuda_fail(e, "attention");
+}
+
 }  // namespace sd
 
 extern "C" {
@@ -1394,16 +1414,7 @@ int sd_attention_dev(const sd_attn_args* a, void* stream) {
     if (rc) return rc;
     if (a->n_tokens == 0) return SD_OK;
     if ((rc = paged_device(a->pool.k, "sd_attention_dev", &dev))) return rc;
-    if (tc_able(*a)) return run_tc(*a, dev, (cudaStream_t)stream);
-    const long long rows = (long long)a->n_tokens * a->n_heads;
-    if ((rows + 3) / 4 > INT32_MAX) return fail(SD_ERR_INVALID, "sd_attention_dev: too many rows");
-    const int grid = (int)((rows + 3) / 4);
-    if (a->pool.dtype == SD_F16)
-        k_pattn_general<__half><<<grid, 128, 0, (cudaStream_t)stream>>>(*a, device_error_word(dev));
-    else
-        k_pattn_general<__nv_bfloat16><<<grid, 128, 0, (cudaStream_t)stream>>>(*a, device_error_word(dev));
-    const cudaError_t e = cudaGetLastError();
-    return e == cudaSuccess ? SD_OK : cuda_fail(e, "attention");
+    return launch_paged_attention(a, dev, device_error_word(dev), (cudaStream_t)stream);
 }
 
 }  // extern "C"

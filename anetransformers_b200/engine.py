@@ -265,13 +265,21 @@ class Context:
 
 class BatchContext:
     """Many independent streams on one GPU sharing a Context's weights (sd_batch_* of the C ABI).  Every
-    stream has its own KV ring and generation state; one forward carries `width` tokens of every stream."""
+    stream has its own KV ring and generation state; one forward carries `width` tokens of every stream.
 
-    def __init__(self, ctx: Context, n_streams: int, max_seq: int, width: int = _lib.BATCH_MAX_WIDTH):
+    With `prefix` (token ids) every stream continues that prompt: its K/V is computed and kept once, read once per
+    forward for all streams, and positions count from its end (sd_batch_create_shared)."""
+
+    def __init__(self, ctx: Context, n_streams: int, max_seq: int, width: int = _lib.BATCH_MAX_WIDTH, prefix=None):
         self.ctx = ctx  # keeps the weights alive
         self.n_streams, self.max_seq, self.width, self.vocab = n_streams, max_seq, width, ctx.vocab
         h = C.c_void_p()
-        _lib.check(_lib.lib().sd_batch_create(ctx.h, n_streams, max_seq, width, C.byref(h)), "sd_batch_create")
+        if prefix is None:
+            _lib.check(_lib.lib().sd_batch_create(ctx.h, n_streams, max_seq, width, C.byref(h)), "sd_batch_create")
+        else:
+            t = _i32(prefix)
+            _lib.check(_lib.lib().sd_batch_create_shared(ctx.h, t.ctypes.data, t.size, n_streams, max_seq, width, C.byref(h)),
+                       "sd_batch_create_shared")
         self.h = h
 
     def close(self):

@@ -90,8 +90,8 @@ class PagePool:
         """Pages and slots of one step (sd_pages_plan_dev): kv_len [n_req] positions after it, q_len [n_req] new ones."""
         n, dev = self._c.n_req, self.table.device
         if out is None:
-            out = Plan(torch.empty(n, dtype=torch.int32, device=dev), torch.empty(n_tokens, dtype=torch.int32, device=dev),
-                       torch.empty(n_tokens, dtype=torch.int32, device=dev), torch.empty(1, dtype=torch.int32, device=dev))
+            buf = torch.empty(n + 2 * n_tokens + 1, dtype=torch.int32, device=dev)
+            out = Plan(*buf.split_with_sizes((n, n_tokens, n_tokens, 1)))
         _call("pages plan", _lib.lib().sd_pages_plan_dev, (self.table, kv_len, q_len, *out), self._ref, _i32("kv_len", kv_len, n),
               _i32("q_len", q_len, n), q_stride, pos0, n_tokens, _i32("q_start", out.q_start, n), _i32("slots", out.slots, n_tokens),
               _i32("positions", out.positions, n_tokens), _i32("missing", out.missing, 1))

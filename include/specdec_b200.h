@@ -213,7 +213,8 @@ typedef struct {
     void *workspace; /* sd_attention_workspace(a) bytes, 256-byte aligned; one call at a time uses it */
     size_t workspace_bytes;
 } sd_attn_args;
-/* Workspace bytes of a call with these sizes (its pointers are not read); 0 may be passed as NULL. */
+/* Workspace bytes of this call (all fields but the workspace set as for it; nothing is dereferenced); for 0 bytes the
+ * workspace may be NULL. */
 SD_API size_t sd_attention_workspace(const sd_attn_args *a);
 SD_API int sd_attention_dev(const sd_attn_args *a, void *stream);
 
@@ -476,6 +477,15 @@ SD_API int sd_batch_set_gemm(sd_batch *b, int mode);
 /* One forward of T <= max_width tokens per stream: tokens [n_streams][T] at positions pos[s] .. pos[s]+T-1
  * (K/V written to each stream's ring); logits: host [n_streams][T][vocab] or NULL. */
 SD_API int sd_batch_forward(sd_batch *b, const int32_t *tokens, int T, const int32_t *pos, float *logits);
+/* A batch whose streams all continue one prompt prefix (a system prompt, few-shot examples, a document): its K/V is
+ * computed here once and kept once, and every forward's attention reads it once for the rows of all streams.  K/V lives
+ * in pages (sd_pages, sd_attention_dev) instead of one ring per stream.  Every sd_batch_* call works on it, counting a
+ * stream's positions from the end of the prefix (position 0 is the first token behind it); max_seq is their number.
+ * A forward gives back the pages of positions behind its last token; a stream's n-gram history and repetition window
+ * do not reach into the prefix.  Logits agree with those of a plain batch over prefix + tokens within the batched path's
+ * tolerance (5e-3 relative): both attend with single fp16 Q and P. */
+SD_API int sd_batch_create_shared(sd_ctx *ctx, const int32_t *prefix, int n_prefix, int n_streams, int max_seq,
+                                  int max_width, sd_batch **out);
 /* K/V of positions [0, n) of every stream from tokens [n_streams][n] (chunks of max_width tokens). */
 SD_API int sd_batch_prefill(sd_batch *b, const int32_t *tokens, int n);
 /* Decode of every stream after a prefill of history[s][0 .. n_hist-1): starts from first[s] at position

@@ -100,3 +100,11 @@ def test_plan_oracle_rules():
     # two pages wanted, one free
     q_start, slots, pos, missing = PO.plan(st, [16, 40, 17], [0, 0, 2], 16, 2)
     assert missing == 1 and st["table"][2] == [4] and slots == [4 * 16 + 15, -1] and pos == [15, 16]
+
+
+def test_shared_batch_refusals():
+    L, out = _lib.lib(), C.c_void_p()
+    for args in [(None, P, 4, 2, 64, 5), (P, None, 4, 2, 64, 5), (P, P, 0, 2, 64, 5), (P, P, 4, 0, 64, 5), (P, P, 4, 2, 15, 5),
+                 (P, P, 4, 2, 64, 0), (P, P, 4, 2, 64, 9), (P, P, 1 << 30, 2, 64, 5)]:
+        refused(L.sd_batch_create_shared(*args, C.byref(out)))
+    refused(L.sd_batch_create_shared(P, P, 4, 2, 64, 5, None))
