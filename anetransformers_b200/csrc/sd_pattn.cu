@@ -132,8 +132,8 @@ __global__ void __launch_bounds__(128) k_pattn_general(const sd_attn_args a, int
 // ones, and slot 0 merges the two states at the end.  Rows whose keys lie in several items leave (max, sum, O) in
 // the workspace for k_pattn_combine; others are written by their item.
 //
-// Warps (12): 0-3 softmax of slot 0, 4-7 of slot 1 (thread = row), 8 TMA, 9 MMA issue, 10 zeroes V rows that no row
-// may see (0 x NaN is NaN in the product), 11 hands out the items.  P overwrites S in tensor memory and is the A operand of P V.
+// Warps (12): 0-3 softmax of slot 0, 4-7 of slot 1 (thread = row), 8 TMA and the handing out of items, 9 and 11 MMA
+// issue of slot 0 and 1, 10 zeroes V rows that no row may see (0 x NaN is NaN in the product).  P overwrites S in tensor memory and is the A operand of P V.
 // The running maximum that O refers to moves only when a row's maximum rises by more than 2^8 (exact: O and the sum
 // refer to the same value), so O is rarely rescaled.  Every wait is bounded in time (sd_common.cuh).
 // ---------------------------------------------------------------------------------------------
@@ -307,14 +307,40 @@ __device__ __forceinline__ bool pa_wait_warp(uint64_t* bar, uint32_t parity, PaC
     return __all_sync(0xffffffffu, pa_wait_slow(bar, parity, ctl, err, code));
 }
 
-// The CTA's k-th item, or -1 after the last (or when a wait ran out).  Ten warps take each item; with the last
-// of them the scheduler warp may hand out the next one.
+// The CTA's k-th item, or -1 after the last (or when a wait ran out), for a warp and for one thread.  Ten take each item;
+// with the last of them the TMA warp may hand out the next one.
 __device__ __forceinline__ int pa_next(PaCtl* ctl, int k, int lane, int* err) {
     if (!pa_wait_warp(&ctl->ifull, k & 1, ctl, err, DEV_ERR_FULL_WAIT)) return -1;
     const int i = *(volatile int*)&ctl->item;
     __syncwarp();
     if (lane == 0) mbar_arrive(&ctl->iempty);
     return i;
+}
+__device__ __forceinline__ int pa_next_thread(PaCtl* ctl, int k, int* err) {
+    if (!pa_wait(&ctl->ifull, k & 1, ctl, err, DEV_ERR_FULL_WAIT)) return -1;
+    const int i = *(volatile int*)&ctl->item;
+    mbar_arrive(&ctl->iempty);
+    return i;
+}
+// Claim a CTA of the grid that has not started (cluster launch control); the answer lands in ctl->claimed.
+__device__ __forceinline__ void pa_claim(PaCtl* ctl) {
+    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+    mbar_arrive_expect_tx(&ctl->claim, 16);
+    asm volatile("clusterlaunchcontrol.try_cancel.async.shared::cta.mbarrier::complete_tx::bytes.b128 [%0], [%1];" ::"r"(
+                     smem_u32(&ctl->claimed)),
+                 "r"(smem_u32(&ctl->claim))
+                 : "memory");
+}
+__device__ __forceinline__ int pa_claimed(PaCtl* ctl) {  // its index, or -1 if there is none left
+    uint32_t got, x;
+    asm volatile(
+        "{\n .reg .pred p;\n .reg .b128 r;\n ld.shared.b128 r, [%2];\n"
+        " clusterlaunchcontrol.query_cancel.is_canceled.pred.b128 p, r;\n selp.u32 %0, 1, 0, p;\n"
+        " mov.u32 %1, 0;\n @p clusterlaunchcontrol.query_cancel.get_first_ctaid::x.b32.b128 %1, r;\n}\n"
+        : "=r"(got), "=r"(x)
+        : "r"(smem_u32(&ctl->claimed))
+        : "memory");
+    return got ? (int)x : -1;
 }
 
 __device__ __forceinline__ void tma_3d(uint32_t dst, const CUtensorMap* m, int x, int y, int z, uint64_t* bar) {
@@ -481,11 +507,11 @@ __global__ void __launch_bounds__(kPaThreads, 1) k_pattn(const __grid_constant__
     if (tid == 0) {
         for (int i = 0; i < 2; ++i) {
             mbar_init(&ctl->qfull[i], 1);
-            mbar_init(&ctl->qempty[i], 1);
+            mbar_init(&ctl->qempty[i], 2);
         }
         for (int i = 0; i < NST; ++i) {
             mbar_init(&ctl->full[i], 1);
-            mbar_init(&ctl->empty[i], 1);
+            mbar_init(&ctl->empty[i], 2);
             mbar_init(&ctl->fixed[i], 1);
         }
         for (int i = 0; i < 16; ++i) mbar_init(&ctl->fq[i], 1);
@@ -499,7 +525,7 @@ __global__ void __launch_bounds__(kPaThreads, 1) k_pattn(const __grid_constant__
         }
         mbar_init(&ctl->mready, 128);
         mbar_init(&ctl->mdone, 128);
-        mbar_init(&ctl->done, 1);
+        mbar_init(&ctl->done, 2);
         mbar_init(&ctl->ifull, 1);
         mbar_init(&ctl->iempty, 10);
         mbar_init(&ctl->claim, 1);
@@ -566,11 +592,39 @@ __global__ void __launch_bounds__(kPaThreads, 1) k_pattn(const __grid_constant__
         const int gk = lane / nhk, jk = lane % nhk;
         const uint32_t dst_k = kvs + jk * kSHalf + gk * box * 128, dst_v = kvs + lane * page_bytes;
         bool ok = true;
+        // The grid has one CTA per item; a running CTA takes over CTAs that have not started, so unequal items even out
+        // over the SMs and set-up is paid once per SM.
+        int next = blockIdx.x < n_items ? (int)blockIdx.x : -1, claims = 0;
+        bool open = false;  // a claim is under way
         for (int k = 0; ok; ++k) {
+            const int i = next;
+            if (lane == 0) {
+                ok = k == 0 || pa_wait(&ctl->iempty, (k - 1) & 1, ctl, p.err, DEV_ERR_EMPTY_WAIT);
+                if (ok) {
+                    *(volatile int*)&ctl->item = i;
+                    mbar_arrive(&ctl->ifull);
+                    if (i >= 0) pa_claim(ctl);
+                }
+            }
+            ok = __shfl_sync(0xffffffffu, ok, 0);
+            if (!ok || i < 0) break;
+            open = true;
+            auto claimed = [&]() {  // the next item
+                do {
+                    if (!open && lane == 0) pa_claim(ctl);
+                    open = true;
+                    ok = pa_wait_warp(&ctl->claim, claims & 1, ctl, p.err, DEV_ERR_FULL_WAIT);
+                    if (!ok) return;
+                    open = false;
+                    ++claims;
+                    next = __shfl_sync(0xffffffffu, pa_claimed(ctl), 0);
+                } while (next >= n_items);
+            };
             PaItem it;
-            const int i = pa_next(ctl, k, lane, p.err);
-            if (i < 0) break;
-            if (!pa_item(p, ustart, i, it) || it.n == 0) continue;
+            if (!pa_item(p, ustart, i, it) || it.n == 0) {
+                claimed();
+                continue;
+            }
             const int* own_table = a.table + (size_t)max(it.b, 0) * a.table_ld;
             auto load_ids = [&](int t) {
                 if (t >= it.n || lane >= npg) return -2;
@@ -660,7 +714,9 @@ __global__ void __launch_bounds__(kPaThreads, 1) k_pattn(const __grid_constant__
                 }
             }
             tiles += it.n;
+            if (ok) claimed();
         }
+        if (open) mbar_wait(&ctl->claim, claims & 1);
         if (lane == 0) {  // the zeroing warp may go
             ctl->fix[fixes & 15] = make_int4(-1, 0, 0, 0);
             mbar_arrive(&ctl->fq[fixes & 15]);
@@ -669,155 +725,117 @@ __global__ void __launch_bounds__(kPaThreads, 1) k_pattn(const __grid_constant__
         for (uint32_t q = pos > NST ? pos - NST : 0; q < pos; ++q) mbar_wait(&ctl->full[q % NST], (q / NST) & 1);
         for (int s = 0; s < 2; ++s)
             if (nq[s] > 0) mbar_wait(&ctl->qfull[s], (nq[s] - 1) & 1);
-    } else if (warp == 9) {
-        // ---------------- MMA issue: the warp walks together, one elected lane issues ----------------
-        constexpr uint32_t id_s = idesc_f16(BF, kPaKeys / 2, false), id_o = idesc_f16(BF, HD, true);
-        const bool leader = elect_one();
-        // 16 keys of V further: within a box [64-element half][row] of up to 64 rows, or in the next page's
-        const uint32_t vbox = min(ps, kPaKeys / 2);
-        uint32_t vstep[4];
+    } else if (warp == 9 || warp == 11) {
+        // ---------------- MMA issue: one elected thread per slot ----------------
+        // A thread's issue of MMAs runs little ahead of the tensor cores, so what it does between them (waits, commits)
+        // would leave them idle; with a thread per slot the other's MMAs fill the gaps.
+        if (elect_one()) {
+            constexpr uint32_t id_s = idesc_f16(BF, kPaKeys / 2, false), id_o = idesc_f16(BF, HD, true);
+            const int slot = warp == 9 ? 0 : 1;
+            uint32_t pos = 0, fixes = 0, tiles = 0, np = 0, nq[2] = {0, 0}, qb = 0;
+            const uint32_t ts = tmem + slot * 128, to = tmem + 256 + slot * HD;
+            // 16 keys of V further: within a box [64-element half][row] of up to 64 rows, or in the next page's
+            const uint32_t vbox = min(ps, kPaKeys / 2);
+            uint32_t vstep[4];
 #pragma unroll
-        for (int ks = 0; ks < 4; ++ks) vstep[ks] = (ks * 16 / vbox * vbox * 128 * NH + ks * 16 % vbox * 128) >> 4;
-        uint32_t pos = 0, fixes = 0, tiles = 0, np[2] = {0, 0}, nq[2] = {0, 0}, qb = 0;
-        bool ok = true;
-        // the next stage of the ring
-        auto wait_stage = [&]() {
-            ok = ok && pa_wait_warp(&ctl->full[pos % NST], (pos / NST) & 1, ctl, p.err, DEV_ERR_FULL_WAIT);
-        };
-        auto commit = [&](uint64_t* bar) {
-            if (leader) pa_commit(bar);
-        };
-        auto release = [&]() {
-            commit(&ctl->empty[pos % NST]);
-            ++pos;
-        };
-        // S of 64 keys: half h of slot's next tile, K in the current stage, against Q tile qt
-        auto score = [&](int slot, int h, int qt) {
-            const uint32_t qa = sw128_lo(qs + qt * TILE, 16), ka = sw128_lo(kvs + (pos % NST) * STAGE, 16);
-            const uint32_t d = tmem + slot * 128 + h * 64;
-            if (leader) {
+            for (int ks = 0; ks < 4; ++ks) vstep[ks] = (ks * 16 / vbox * vbox * 128 * NH + ks * 16 % vbox * 128) >> 4;
+            bool ok = true;
+            // Both threads walk every stage of the ring, in order, and both release it: a parity wait tells a phase from
+            // its neighbour only, so neither may fall a lap behind or get one ahead.
+            auto wait_stage = [&]() {
+                ok = ok && pa_wait(&ctl->full[pos % NST], (pos / NST) & 1, ctl, p.err, DEV_ERR_FULL_WAIT);
+            };
+            // S of 64 keys: half h of the slot's next tile, K in the current stage, against Q
+            auto score = [&](int h, uint32_t qa) {
+                wait_stage();
+                if (!ok) return;
+                const uint32_t ka = sw128_lo(kvs + (pos % NST) * STAGE, 16);
 #pragma unroll
                 for (int ks = 0; ks < HD / 16; ++ks)
-                    mma_ss(d, qa + (((ks >> 2) * kPaHalf + (ks & 3) * 32) >> 4), ka + (((ks >> 2) * kSHalf + (ks & 3) * 32) >> 4), id_s,
-                           ks > 0);
+                    mma_ss(ts + h * 64, qa + (((ks >> 2) * kPaHalf + (ks & 3) * 32) >> 4), ka + (((ks >> 2) * kSHalf + (ks & 3) * 32) >> 4),
+                           id_s, ks > 0);
                 pa_commit(&ctl->sfull[slot][h]);
-            }
-        };
-        // V of half h of tile t in the current stage, its unseen rows zero
-        auto wait_v = [&](int t, int h) {
-            wait_stage();
-            if (ok && (*(volatile uint32_t*)&ctl->okmask[(tiles + t) & 15][h] & 256u)) {
-                ok = pa_wait_warp(&ctl->fixed[pos % NST], fixes >> (pos % NST) & 1, ctl, p.err, DEV_ERR_FULL_WAIT);
-                fixes ^= 1u << (pos % NST);
-            }
-        };
-        // O += P V over 64 keys (V in the current stage), once their P is there
-        auto value = [&](int slot, int h, bool acc, bool last) {
-            const uint32_t va = sw128_lo(kvs + (pos % NST) * STAGE, vbox * 128);
-            const uint32_t d = tmem + 256 + slot * HD, pa = tmem + slot * 128 + h * 64;
-            ok = ok && pa_wait_warp(&ctl->pready[slot][h], np[slot] & 1, ctl, p.err, DEV_ERR_FULL_WAIT);
-            if (!ok) return;
-            pa_fence_after();
-            if (leader) {
-#pragma unroll
-                for (int ks = 0; ks < 4; ++ks) mma_ts(d, pa + ks * 8, va + vstep[ks], id_o, acc || h > 0 || ks > 0);
-                pa_commit(&ctl->ofull[slot]);
-                if (last && h == 1) pa_commit(&ctl->odone[slot]);
-            }
-            if (h == 1) ++np[slot];
-        };
-        for (int k = 0;; ++k) {
-            PaItem it;
-            const int i = pa_next(ctl, k, lane, p.err);
-            if (i < 0) break;
-            if (!pa_item(p, ustart, i, it) || it.n == 0) continue;
-            const int q0 = it.pair ? 0 : (int)qb;
-            for (int s = q0; s <= (it.pair ? 1 : q0); ++s) {
-                ok = ok && pa_wait_warp(&ctl->qfull[s], nq[s] & 1, ctl, p.err, DEV_ERR_FULL_WAIT);
-                ++nq[s];
-            }
-            if (!it.pair) qb ^= 1;
-            if (!ok) break;
-            auto q_done = [&]() {
-                commit(&ctl->qempty[q0]);
-                if (it.pair) commit(&ctl->qempty[1]);
+                pa_commit(&ctl->empty[pos % NST]);
+                ++pos;
             };
-            const int n = it.n;
-            // Half tiles of K and V go through the ring in the order of their use: K of the first tile (of the first two of a
-            // single item, one per slot), then V of tile t and K of the tile that follows it on its slot, half by half.
-            // Each 64-key half of a slot's tile is a buffer of its own: its next S follows its product at once, while the
-            // softmax is at the other half (and the other slot).
-            if (it.pair) {
-#pragma unroll
-                for (int h = 0; h < 2; ++h) {
-                    wait_stage();
-                    if (!ok) break;
-                    score(0, h, 0);
-                    score(1, h, 1);
-                    release();
+            // O += P V over 64 keys (V in the current stage), once V, its unseen rows zero, and P are there
+            auto value = [&](int t, int h, bool acc, bool last) {
+                wait_stage();
+                if (ok && (*(volatile uint32_t*)&ctl->okmask[(tiles + t) & 15][h] & 256u)) {
+                    ok = pa_wait(&ctl->fixed[pos % NST], fixes >> (pos % NST) & 1, ctl, p.err, DEV_ERR_FULL_WAIT);
+                    fixes ^= 1u << (pos % NST);
                 }
-                if (n == 1 && ok) q_done();
+                ok = ok && pa_wait(&ctl->pready[slot][h], np & 1, ctl, p.err, DEV_ERR_FULL_WAIT);
+                if (!ok) return;
+                pa_fence_after();
+                const uint32_t va = sw128_lo(kvs + (pos % NST) * STAGE, vbox * 128);
+#pragma unroll
+                for (int ks = 0; ks < 4; ++ks) mma_ts(to, ts + h * 64 + ks * 8, va + vstep[ks], id_o, acc || h > 0 || ks > 0);
+                pa_commit(&ctl->ofull[slot]);
+                pa_commit(&ctl->empty[pos % NST]);
+                if (last && h == 1) pa_commit(&ctl->odone[slot]);
+                if (h == 1) ++np;
+                ++pos;
+            };
+            // a stage of the other slot's
+            auto pass = [&](bool v, int t, int h) {
+                wait_stage();
+                if (!ok) return;
+                if (v && (*(volatile uint32_t*)&ctl->okmask[(tiles + t) & 15][h] & 256u)) fixes ^= 1u << (pos % NST);
+                mbar_arrive(&ctl->empty[pos % NST]);
+                ++pos;
+            };
+            for (int k = 0; ok; ++k) {
+                PaItem it;
+                const int i = pa_next_thread(ctl, k, p.err);
+                if (i < 0) break;
+                if (!pa_item(p, ustart, i, it) || it.n == 0) continue;
+                // Half tiles of K and V go through the ring in the order of their use: K of the first tile (of the first
+                // two of a single item, one per slot), then V of tile t and K of the tile that follows it on its slot,
+                // half by half.  Each 64-key half of a slot's tile is an S buffer of its own: its next S follows its
+                // product at once, while the softmax is at the other half.
+                const int n = it.n, D = it.pair ? 1 : 2, qt = it.pair ? slot : (int)qb;
+                ok = pa_wait(&ctl->qfull[qt], nq[qt] & 1, ctl, p.err, DEV_ERR_FULL_WAIT);
+                const uint32_t qa = sw128_lo(qs + qt * TILE, 16);
+                auto mine = [&](int t) { return it.pair || (t & 1) == slot; };
+                auto q_done = [&]() {  // two arrivals: this thread's twice, or each slot's once
+                    pa_commit(&ctl->qempty[qt]);
+                    if (it.pair || n == 1) pa_commit(&ctl->qempty[qt]);
+                };
+                for (int t = 0; t < D && t < n; ++t)
+#pragma unroll
+                    for (int h = 0; h < 2 && ok; ++h) {
+                        if (mine(t)) score(h, qa);
+                        else pass(false, t, h);
+                    }
+                const int first = it.pair ? 0 : slot;
+                if (ok && first < n && first + D >= n) q_done();
                 for (int t = 0; t < n && ok; ++t) {
-                    const bool more = t + 1 < n;
+                    const bool more = t + D < n, own = mine(t);
 #pragma unroll
-                    for (int h = 0; h < 2; ++h) {
-                        // V is in the current stage, K of the next tile in the one behind it
-                        wait_v(t, h);
-                        value(0, h, t > 0, !more);
-                        if (!ok) break;
-                        if (more) {
-                            ++pos;
-                            wait_stage();
-                            if (!ok) break;
-                            score(0, h, 0);
-                            --pos;
-                        }
-                        value(1, h, t > 0, !more);
-                        if (!ok) break;
-                        release();
-                        if (more) {
-                            score(1, h, 1);
-                            release();
+                    for (int h = 0; h < 2 && ok; ++h) {
+                        if (own) value(t, h, t >= D, !more);
+                        else pass(true, t, h);
+                        if (more && ok) {
+                            if (own) score(h, qa);
+                            else pass(false, t + D, h);
                         }
                     }
-                    if (t + 2 == n && ok) q_done();
+                    if (own && more && t + 2 * D >= n && ok) q_done();
                 }
-            } else {
-#pragma unroll
-                for (int s = 0; s < 2; ++s)
-#pragma unroll
-                    for (int h = 0; h < 2; ++h) {
-                        if (s >= n || !ok) break;
-                        wait_stage();
-                        if (!ok) break;
-                        score(s, h, q0);
-                        release();
-                    }
-                if (n <= 2 && ok) q_done();
-                for (int t = 0; t < n && ok; ++t) {
-                    const bool more = t + 2 < n;
-#pragma unroll
-                    for (int h = 0; h < 2; ++h) {
-                        wait_v(t, h);
-                        value(t & 1, h, t > 1, !more);
-                        if (!ok) break;
-                        release();
-                        if (more) {
-                            wait_stage();
-                            if (!ok) break;
-                            score(t & 1, h, q0);
-                            release();
-                        }
-                    }
-                    if (t + 3 == n && ok) q_done();
+                if (it.pair) {
+                    ++nq[0];
+                    ++nq[1];
+                } else {
+                    ++nq[qb];
+                    qb ^= 1;
                 }
+                tiles += n;
             }
-            tiles += n;
-            if (!ok) break;
+            // every MMA issued above has completed before the tensor memory is released
+            pa_commit(&ctl->done);
+            if (!mbar_wait(&ctl->done, 0)) set_dev_error(p.err, DEV_ERR_FULL_WAIT);
         }
-        // every MMA issued above has completed before the tensor memory is released
-        commit(&ctl->done);
-        if (!mbar_wait(&ctl->done, 0)) set_dev_error(p.err, DEV_ERR_FULL_WAIT);
         __syncwarp();
     } else if (warp == 10) {
         // ---------------- V rows that no row of the item may see become zero ----------------
@@ -842,43 +860,6 @@ __global__ void __launch_bounds__(kPaThreads, 1) k_pattn(const __grid_constant__
             __syncwarp();
             if (lane == 0) mbar_arrive(&ctl->fixed[f.x]);
         }
-    } else if (warp == 11) {
-        // ---------------- scheduler ----------------
-        // The grid has one CTA per item; a running CTA takes over CTAs that have not started (cluster launch
-        // control), so unequal items even out over the SMs and set-up is paid once per SM.
-        if (lane == 0) {
-            int i = blockIdx.x < n_items ? (int)blockIdx.x : -1, claims = 0;
-            for (int k = 0;; ++k) {
-                if (k > 0 && !pa_wait(&ctl->iempty, (k - 1) & 1, ctl, p.err, DEV_ERR_EMPTY_WAIT)) break;
-                *(volatile int*)&ctl->item = i;
-                mbar_arrive(&ctl->ifull);
-                if (i < 0) break;
-                do {
-                    mbar_arrive_expect_tx(&ctl->claim, 16);
-                    asm volatile("clusterlaunchcontrol.try_cancel.async.shared::cta.mbarrier::complete_tx::bytes.b128 [%0], [%1];" ::"r"(
-                                     smem_u32(&ctl->claimed)),
-                                 "r"(smem_u32(&ctl->claim))
-                                 : "memory");
-                    if (!mbar_wait(&ctl->claim, claims & 1)) {
-                        set_dev_error(p.err, DEV_ERR_FULL_WAIT);
-                        *(volatile int*)&ctl->abort = 1;
-                    }
-                    ++claims;
-                    uint32_t got, x;
-                    asm volatile(
-                        "{\n .reg .pred p;\n .reg .b128 r;\n ld.shared.b128 r, [%2];\n"
-                        " clusterlaunchcontrol.query_cancel.is_canceled.pred.b128 p, r;\n selp.u32 %0, 1, 0, p;\n"
-                        " mov.u32 %1, 0;\n @p clusterlaunchcontrol.query_cancel.get_first_ctaid::x.b32.b128 %1, r;\n}\n"
-                        : "=r"(got), "=r"(x)
-                        : "r"(smem_u32(&ctl->claimed))
-                        : "memory");
-                    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-                    i = got ? (int)x : -1;
-                } while (i >= n_items && !*(volatile int*)&ctl->abort);
-                if (*(volatile int*)&ctl->abort) i = -1;
-            }
-        }
-        __syncwarp();
     } else {
         // ---------------- softmax: thread = row of its slot ----------------
         const int slot = warp >> 2, row = tid & 127;
