@@ -19,21 +19,6 @@
 
 using namespace sd;
 
-#ifndef PA_MIN
-#define PA_MIN 4
-#endif
-#ifndef PA_OV
-#define PA_OV 1.0
-#endif
-#ifndef PA_PMIN
-#define PA_PMIN 4
-#endif
-#ifndef PA_PR
-#define PA_PR 1
-#endif
-#ifndef PA_POLY
-#define PA_POLY 0
-#endif
 namespace sd {
 namespace {
 
@@ -437,32 +422,20 @@ __device__ __forceinline__ float rcp(float x) {
     asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
     return y;
 }
-// 2^z of two values on the FMA pipe: z = i + f with i the nearest integer (added to 1.5 2^23 it stands in the low
-// mantissa bits), 2^f by a polynomial of degree 4 on [-1/2, 1/2] with constant term 1 (minimax, relative error
-// 2.8e-6), i added to the exponent.  Below -127 the result is 0.
-__device__ __forceinline__ float2 ex2_fma(float2 z) {
-    z.x = fmaxf(z.x, -127.f);
-    z.y = fmaxf(z.y, -127.f);
-    const float2 t = __fadd2_rn(z, make_float2(12582912.f, 12582912.f));
-    const float2 f = __fadd2_rn(z, __ffma2_rn(t, make_float2(-1.f, -1.f), make_float2(12582912.f, 12582912.f)));
-    float2 q = __ffma2_rn(f, make_float2(0.009582852944731712f, 0.009582852944731712f),
-                          make_float2(0.055906426161527634f, 0.055906426161527634f));
-    q = __ffma2_rn(f, q, make_float2(0.24024099111557007f, 0.24024099111557007f));
-    q = __ffma2_rn(f, q, make_float2(0.6931241750717163f, 0.6931241750717163f));
-    q = __ffma2_rn(f, q, make_float2(1.f, 1.f));
-    return make_float2(__uint_as_float(__float_as_uint(q.x) + (__float_as_uint(t.x) << 23)),
-                       __uint_as_float(__float_as_uint(q.y) + (__float_as_uint(t.y) << 23)));
+// cap tanh(x) of two values with |x| <= 1/2: x times a polynomial in x^2 (minimax, relative error 6.4e-7) times the cap.
+struct CapPoly {
+    float2 c0, c1, c2, c3;
+};
+__device__ __forceinline__ CapPoly cap_poly(float cap) {
+    const float a = -0.33328160643577576f * cap, b = 0.13205359876155853f * cap, c = -0.0447506457567215f * cap;
+    return CapPoly{make_float2(cap, cap), make_float2(a, a), make_float2(b, b), make_float2(c, c)};
 }
-// tanh of two values in [-1, 1]: x times a polynomial in x^2 (minimax, relative error 5.5e-8).
-__device__ __forceinline__ float2 tanh_small(float2 x) {
+__device__ __forceinline__ float2 cap_small(float2 x, const CapPoly& k) {
     const float2 u = __fmul2_rn(x, x);
-    float2 q = make_float2(0.0010582432f, 0.0010582432f);
-    q = __ffma2_rn(u, q, make_float2(-0.0062592784f, -0.0062592784f));
-    q = __ffma2_rn(u, q, make_float2(0.020359693f, 0.020359693f));
-    q = __ffma2_rn(u, q, make_float2(-0.053498674f, -0.053498674f));
-    q = __ffma2_rn(u, q, make_float2(0.13326408f, 0.13326408f));
-    q = __ffma2_rn(u, q, make_float2(-0.33332986f, -0.33332986f));
-    return __ffma2_rn(__fmul2_rn(x, u), q, x);
+    float2 q = __ffma2_rn(u, k.c3, k.c2);
+    q = __ffma2_rn(u, q, k.c1);
+    q = __ffma2_rn(u, q, k.c0);
+    return __fmul2_rn(x, q);
 }
 template <class T> __device__ __forceinline__ uint32_t pa_pack(float lo, float hi);
 template <> __device__ __forceinline__ uint32_t pa_pack<__half>(float lo, float hi) {
@@ -495,7 +468,6 @@ __global__ void __launch_bounds__(kPaThreads, 1) k_pattn(const __grid_constant__
     // ones stay in the type's normal range
     constexpr float kShift = BF ? 0.f : 6.f;
     constexpr float kSlack = 8.f;
-    constexpr int POLY = PA_POLY;
     extern __shared__ uint8_t raw[];
     uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(raw) + 1023) & ~(uintptr_t)1023);
     const uint32_t qs = smem_u32(smem), kvs = qs + 2 * TILE;
@@ -870,6 +842,7 @@ __global__ void __launch_bounds__(kPaThreads, 1) k_pattn(const __grid_constant__
         const float sc2 = a.scale * kLog2e;
         // capped: cap log2e tanh(x) with x = scale s / cap, as cap log2e (1 - 2 / (1 + 2^(2 log2e x)))
         const float cap2 = a.softcap * kLog2e, x1 = a.softcap > 0.f ? a.scale / a.softcap : 0.f;
+        const CapPoly kcap = cap_poly(cap2);
         uint32_t ns = 0, np = 0, nd = 0, nm = 0, tiles = 0;  // phases of sfull, ofull, odone and the merges; key tiles so far
         bool ok = true;
         for (int k = 0; ok; ++k) {
@@ -924,22 +897,21 @@ __global__ void __launch_bounds__(kPaThreads, 1) k_pattn(const __grid_constant__
                         pa_wait_ld(y[1]);
                         if (MOD) {
                             if (a.softcap > 0.f) {
-                                // scores below the cap (nearly all): tanh without the special function unit, which the
-                                // weights' exp2 already fills
+                                // scores below half the cap (nearly all): tanh without the special function unit, which
+                                // the weights' exp2 already fills
                                 float big = 0.f;
 #pragma unroll
                                 for (int c = 0; c < 2; ++c)
 #pragma unroll
                                     for (int e = 0; e < 32; e += 2)
                                         big = fmaxf(big, fmaxf(fabsf(__uint_as_float(y[c][e])), fabsf(__uint_as_float(y[c][e + 1]))));
-                                if (__all_sync(0xffffffffu, big * fabsf(x1) <= 1.f)) {
+                                if (__all_sync(0xffffffffu, big * fabsf(x1) <= 0.5f)) {
 #pragma unroll
                                     for (int c = 0; c < 2; ++c)
 #pragma unroll
                                         for (int e = 0; e < 32; e += 2) {
-                                            const float2 x = __fmul2_rn(make_float2(__uint_as_float(y[c][e]), __uint_as_float(y[c][e + 1])),
-                                                                        make_float2(x1, x1));
-                                            const float2 z = __fmul2_rn(tanh_small(x), make_float2(cap2, cap2));
+                                            const float2 z = cap_small(__fmul2_rn(make_float2(__uint_as_float(y[c][e]), __uint_as_float(y[c][e + 1])),
+                                                                                  make_float2(x1, x1)), kcap);
                                             y[c][e] = __float_as_uint(z.x);
                                             y[c][e + 1] = __float_as_uint(z.y);
                                         }
@@ -950,26 +922,28 @@ __global__ void __launch_bounds__(kPaThreads, 1) k_pattn(const __grid_constant__
                                         for (int e = 0; e < 32; e += 2) {
                                             const float2 x = __fmul2_rn(make_float2(__uint_as_float(y[c][e]), __uint_as_float(y[c][e + 1])),
                                                                         make_float2(x1, x1));
-                                            float2 z = __fmul2_rn(tanh_small(x), make_float2(cap2, cap2));
-                                            if (!(fabsf(x.x) <= 1.f)) z.x = fmaf(rcp(1.f + ex2(x.x * (2.f * kLog2e))), -2.f * cap2, cap2);
-                                            if (!(fabsf(x.y) <= 1.f)) z.y = fmaf(rcp(1.f + ex2(x.y * (2.f * kLog2e))), -2.f * cap2, cap2);
+                                            float2 z = cap_small(x, kcap);
+                                            if (!(fabsf(x.x) <= 0.5f)) z.x = fmaf(rcp(1.f + ex2(x.x * (2.f * kLog2e))), -2.f * cap2, cap2);
+                                            if (!(fabsf(x.y) <= 0.5f)) z.y = fmaf(rcp(1.f + ex2(x.y * (2.f * kLog2e))), -2.f * cap2, cap2);
                                             y[c][e] = __float_as_uint(z.x);
                                             y[c][e + 1] = __float_as_uint(z.y);
                                         }
                                 }
-                            } else {
-#pragma unroll
-                                for (int c = 0; c < 2; ++c)
-#pragma unroll
-                                    for (int e = 0; e < 32; ++e) y[c][e] = __float_as_uint(__uint_as_float(y[c][e]) * sc2);
                             }
-                            if (a.alibi) {
+                            // z = (capped, or scale log2e s) - slope distance, the distance of key e being (own - k0) - e
+                            if (a.alibi || !(a.softcap > 0.f)) {
                                 const float bias = slope * (float)((kt.prefix ? P : 0) + own - k0);
+                                const float f = a.softcap > 0.f ? 1.f : sc2;
+                                const float2 f2 = make_float2(f, f), s2 = make_float2(slope, slope), b2 = make_float2(-bias, -bias);
 #pragma unroll
                                 for (int c = 0; c < 2; ++c)
 #pragma unroll
-                                    for (int e = 0; e < 32; ++e)
-                                        y[c][e] = __float_as_uint(__uint_as_float(y[c][e]) + fmaf(slope, (float)(c * 32 + e), -bias));
+                                    for (int e = 0; e < 32; e += 2) {
+                                        const float2 add = __ffma2_rn(s2, make_float2((float)(c * 32 + e), (float)(c * 32 + e + 1)), b2);
+                                        const float2 z = __ffma2_rn(make_float2(__uint_as_float(y[c][e]), __uint_as_float(y[c][e + 1])), f2, add);
+                                        y[c][e] = __float_as_uint(z.x);
+                                        y[c][e + 1] = __float_as_uint(z.y);
+                                    }
                             }
                         }
                         if (!whole) {
@@ -1022,12 +996,8 @@ __global__ void __launch_bounds__(kPaThreads, 1) k_pattn(const __grid_constant__
                         for (int e = 0; e < 32; ++e) {
                             float2 z = __ffma2_rn(make_float2(__uint_as_float(y[e >> 4][(e & 15) * 2]), __uint_as_float(y[e >> 4][(e & 15) * 2 + 1])),
                                                   one2, ref2);
-                            if (POLY && e % (POLY ? POLY : 1) == POLY - 1) {
-                                z = ex2_fma(z);
-                            } else {
-                                z.x = ex2(z.x);
-                                z.y = ex2(z.y);
-                            }
+                            z.x = ex2(z.x);
+                            z.y = ex2(z.y);
                             sum[e & 1] = __fadd2_rn(sum[e & 1], z);
                             pk[e] = pa_pack<T>(z.x, z.y);
                         }
@@ -1223,10 +1193,10 @@ void pa_plan(const sd_attn_args& a, int sms, PaArgs* p) {
     const int seen = a.window > 0 ? (int)std::min<long long>(own, ((long long)a.window + std::min(a.max_q, pair)) / kPaKeys + 2) : own;
     int ct = std::max(seen, 1);
     if (a.max_q <= p->TPT) {
-        // few rows per item: a chunk costs about PA_OV tiles to start and to join, and the last one to end leaves the
-        // other SMs idle for up to its length: the sum is least at the square root of PA_OV times an SM's tiles
+        // few rows per item: a chunk costs about one tile to start and to join, and the last one to end leaves the
+        // other SMs idle for up to its length: the sum is least at the square root of an SM's tiles
         const double per_sm = (double)units * seen / sms;
-        ct = std::max(PA_MIN, (int)(std::sqrt(PA_OV * per_sm) + 0.5));
+        ct = std::max(4, (int)(std::sqrt(per_sm) + 0.5));
     } else {
         // many rows: whole rounds over the SMs; a cut costs about 3 tiles more (O of 256 rows in 32 bits, twice)
         double best = 1e300;
@@ -1243,7 +1213,7 @@ void pa_plan(const sd_attn_args& a, int sms, PaArgs* p) {
     p->cp = 0;
     if (p->np) {
         const long long u = (long long)n_kv * p->n_pt;
-        const long long n = std::max<long long>(1, std::min<long long>((p->np + PA_PMIN - 1) / PA_PMIN, (long long)PA_PR * sms / u));
+        const long long n = std::max<long long>(1, std::min<long long>((p->np + 3) / 4, sms / u));
         p->ct_pre = (int)((p->np + n - 1) / n);
         p->cp = (p->np + p->ct_pre - 1) / p->ct_pre;
     }
