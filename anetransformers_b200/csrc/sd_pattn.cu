@@ -133,9 +133,21 @@ struct PaArgs {
     int np;                // key tiles of the prefix
     int n_pt, cp, ct_pre;  // prefix items: row-tile pairs over the tokens, chunks, tiles per chunk
     int ct_own;            // tiles per chunk of own items
-    float* acc;            // [splits][n_tokens * n_heads][hd]
-    float2* ml;            // [splits][n_tokens * n_heads]
+    // States of rows whose keys lie in several items, by split; row (kv head, token, head of its group), so that the rows
+    // of a tile, one per thread, are neighbours: O as float4 [splits][hd / 4][rows], (max, sum) as [splits][rows].
+    float4* acc;
+    float2* ml;
     int* err;
+};
+
+struct alignas(16) PaItem {
+    int b, kvh, tok0, ntok;   // request (-1: prefix item), kv head, first token, tokens
+    int pair, direct;
+    int v0, n, npt;           // first key tile, their number; tiles below npt are the prefix's
+    int klo_p, klo_o, khi_o;  // keys outside [klo_p, prefix_len) and [klo_o, khi_o) are seen by no row of the item
+    int base;                 // kv - q: own position of the request's first row
+    int q0, rows;             // the request's first token and its tokens
+    int split;
 };
 
 struct PaCtl {
@@ -148,7 +160,7 @@ struct PaCtl {
     uint64_t mready, mdone, done;
     uint64_t ifull, iempty, claim;  // hand-over of the next item; answer to the claim of another CTA's
     uint4 claimed;
-    int item;
+    PaItem item;  // ntok 0: no more
     // per key tile (in turn) and half: which of its 16-key groups were loaded (bits 0-3), and whether V has rows that no
     // row of the item may see (bit 8)
     uint32_t okmask[16][2];
@@ -159,16 +171,6 @@ struct PaCtl {
     uint32_t tmem;
     int abort;
     int wsum[16];
-};
-
-struct PaItem {
-    int b, kvh, tok0, ntok;   // request (-1: prefix item), kv head, first token, tokens
-    bool pair, direct;
-    int v0, n, npt;           // first key tile, their number; tiles below npt are the prefix's
-    int klo_p, klo_o, khi_o;  // keys outside [klo_p, prefix_len) and [klo_o, khi_o) are seen by no row of the item
-    int base;                 // kv - q: own position of the request's first row
-    int q0, rows;             // the request's first token and its tokens
-    int split;
 };
 
 __device__ __forceinline__ int pa_q(const sd_attn_args& a, int b) { return min(max(a.q_len[b], 0), a.max_q); }
@@ -197,7 +199,8 @@ __device__ __forceinline__ int pa_request(const sd_attn_args& a, int tok) {
     return lo;
 }
 
-// Item number i of the launch; false if it holds nothing (prefix rows of an inline request).
+// Item number i of the launch; false if it holds nothing (prefix rows of an inline request).  The TMA warp does this, ahead
+// of the others; they read the result.
 __device__ __forceinline__ bool pa_item(const PaArgs& p, const int* ustart, int i, PaItem& it) {
     const sd_attn_args& a = p.a;
     const int n_kv = a.pool.n_kv_heads, P = a.prefix_len, W = a.window;
@@ -292,20 +295,20 @@ __device__ __forceinline__ bool pa_wait_warp(uint64_t* bar, uint32_t parity, PaC
     return __all_sync(0xffffffffu, pa_wait_slow(bar, parity, ctl, err, code));
 }
 
-// The CTA's k-th item, or -1 after the last (or when a wait ran out), for a warp and for one thread.  Ten take each item;
+// The CTA's k-th item, for a warp and for one thread; false after the last (or when a wait ran out).  Ten take each item;
 // with the last of them the TMA warp may hand out the next one.
-__device__ __forceinline__ int pa_next(PaCtl* ctl, int k, int lane, int* err) {
-    if (!pa_wait_warp(&ctl->ifull, k & 1, ctl, err, DEV_ERR_FULL_WAIT)) return -1;
-    const int i = *(volatile int*)&ctl->item;
+__device__ __forceinline__ bool pa_next(PaCtl* ctl, int k, int lane, int* err, PaItem& it) {
+    if (!pa_wait_warp(&ctl->ifull, k & 1, ctl, err, DEV_ERR_FULL_WAIT)) return false;
+    it = ctl->item;
     __syncwarp();
     if (lane == 0) mbar_arrive(&ctl->iempty);
-    return i;
+    return it.ntok > 0;
 }
-__device__ __forceinline__ int pa_next_thread(PaCtl* ctl, int k, int* err) {
-    if (!pa_wait(&ctl->ifull, k & 1, ctl, err, DEV_ERR_FULL_WAIT)) return -1;
-    const int i = *(volatile int*)&ctl->item;
+__device__ __forceinline__ bool pa_next_thread(PaCtl* ctl, int k, int* err, PaItem& it) {
+    if (!pa_wait(&ctl->ifull, k & 1, ctl, err, DEV_ERR_FULL_WAIT)) return false;
+    it = ctl->item;
     mbar_arrive(&ctl->iempty);
-    return i;
+    return it.ntok > 0;
 }
 // Claim a CTA of the grid that has not started (cluster launch control); the answer lands in ctl->claimed.
 __device__ __forceinline__ void pa_claim(PaCtl* ctl) {
@@ -544,6 +547,7 @@ __global__ void __launch_bounds__(kPaThreads, 1) k_pattn(const __grid_constant__
     pa_fence_before();
     __syncthreads();
     pa_fence_after();
+    pdl_trigger();
     const uint32_t tmem = ctl->tmem;
     const int n_items = (p.cp * p.n_pt + ustart[a.n_req]) * a.pool.n_kv_heads;
     const int ps = a.pool.page_size, G = p.G;
@@ -568,32 +572,39 @@ __global__ void __launch_bounds__(kPaThreads, 1) k_pattn(const __grid_constant__
         // over the SMs and set-up is paid once per SM.
         int next = blockIdx.x < n_items ? (int)blockIdx.x : -1, claims = 0;
         bool open = false;  // a claim is under way
-        for (int k = 0; ok; ++k) {
-            const int i = next;
+        auto claimed = [&]() {  // the next item's number
+            do {
+                if (!open && lane == 0) pa_claim(ctl);
+                open = true;
+                ok = pa_wait_warp(&ctl->claim, claims & 1, ctl, p.err, DEV_ERR_FULL_WAIT);
+                if (!ok) return;
+                open = false;
+                ++claims;
+                next = __shfl_sync(0xffffffffu, pa_claimed(ctl), 0);
+            } while (next >= n_items);
+        };
+        for (int k = 0; ok;) {
+            PaItem it;
+            it.ntok = 0;
+            if (next >= 0) {
+                if (lane == 0) pa_claim(ctl);
+                open = true;
+                if (!pa_item(p, ustart, next, it)) {
+                    claimed();
+                    continue;
+                }
+            }
             if (lane == 0) {
                 ok = k == 0 || pa_wait(&ctl->iempty, (k - 1) & 1, ctl, p.err, DEV_ERR_EMPTY_WAIT);
                 if (ok) {
-                    *(volatile int*)&ctl->item = i;
+                    ctl->item = it;
                     mbar_arrive(&ctl->ifull);
-                    if (i >= 0) pa_claim(ctl);
                 }
             }
+            ++k;
             ok = __shfl_sync(0xffffffffu, ok, 0);
-            if (!ok || i < 0) break;
-            open = true;
-            auto claimed = [&]() {  // the next item
-                do {
-                    if (!open && lane == 0) pa_claim(ctl);
-                    open = true;
-                    ok = pa_wait_warp(&ctl->claim, claims & 1, ctl, p.err, DEV_ERR_FULL_WAIT);
-                    if (!ok) return;
-                    open = false;
-                    ++claims;
-                    next = __shfl_sync(0xffffffffu, pa_claimed(ctl), 0);
-                } while (next >= n_items);
-            };
-            PaItem it;
-            if (!pa_item(p, ustart, i, it) || it.n == 0) {
+            if (!ok || it.ntok == 0) break;
+            if (it.n == 0) {
                 claimed();
                 continue;
             }
@@ -759,9 +770,8 @@ __global__ void __launch_bounds__(kPaThreads, 1) k_pattn(const __grid_constant__
             };
             for (int k = 0; ok; ++k) {
                 PaItem it;
-                const int i = pa_next_thread(ctl, k, p.err);
-                if (i < 0) break;
-                if (!pa_item(p, ustart, i, it) || it.n == 0) continue;
+                if (!pa_next_thread(ctl, k, p.err, it)) break;
+                if (it.n == 0) continue;
                 // Half tiles of K and V go through the ring in the order of their use: K of the first tile (of the first
                 // two of a single item, one per slot), then V of tile t and K of the tile that follows it on its slot,
                 // half by half.  Each 64-key half of a slot's tile is an S buffer of its own: its next S follows its
@@ -847,9 +857,7 @@ __global__ void __launch_bounds__(kPaThreads, 1) k_pattn(const __grid_constant__
         bool ok = true;
         for (int k = 0; ok; ++k) {
             PaItem it;
-            const int i = pa_next(ctl, k, lane, p.err);
-            if (i < 0) break;
-            if (!pa_item(p, ustart, i, it)) continue;
+            if (!pa_next(ctl, k, lane, p.err, it)) break;
             const int tok = it.tok0 + (it.pair ? slot * p.TPT : 0) + row_tok;
             const int head = it.kvh * G + row_head;
             const bool live = row_tok < p.TPT && tok < it.tok0 + it.ntok;
@@ -1041,8 +1049,8 @@ __global__ void __launch_bounds__(kPaThreads, 1) k_pattn(const __grid_constant__
                 }
             }
             if ((it.pair || slot == 0) && !idle) {
-                const size_t orow = (size_t)tok * a.n_heads + head;
-                const size_t prow = (size_t)it.split * a.n_tokens * a.n_heads + orow;
+                const size_t ld = (size_t)a.n_tokens * a.n_heads;
+                const size_t prow = ((size_t)it.kvh * a.n_tokens + tok) * G + row_head;
                 const float inv = l > 0.f ? 1.f / l : (l == 0.f ? 0.f : l);  // NaN stays NaN
 #pragma unroll 1
                 for (int c = 0; c < HD / 32; ++c) {
@@ -1072,14 +1080,14 @@ __global__ void __launch_bounds__(kPaThreads, 1) k_pattn(const __grid_constant__
 #pragma unroll
                         for (int e = 0; e < 4; ++e) dst[e] = make_uint4(pk[4 * e], pk[4 * e + 1], pk[4 * e + 2], pk[4 * e + 3]);
                     } else {
-                        float4* dst = reinterpret_cast<float4*>(p.acc + prow * HD + c * 32);
+                        float4* dst = p.acc + ((size_t)it.split * (HD / 4) + c * 8) * ld + prow;
 #pragma unroll
                         for (int e = 0; e < 8; ++e)
-                            dst[e] = make_float4(__uint_as_float(o[4 * e]), __uint_as_float(o[4 * e + 1]), __uint_as_float(o[4 * e + 2]),
+                            dst[e * ld] = make_float4(__uint_as_float(o[4 * e]), __uint_as_float(o[4 * e + 1]), __uint_as_float(o[4 * e + 2]),
                                                  __uint_as_float(o[4 * e + 3]));
                     }
                 }
-                if (!it.direct && live) p.ml[prow] = make_float2(m, l);
+                if (!it.direct && live) p.ml[it.split * ld + prow] = make_float2(m, l);
             }
             if (merge) {
                 if (slot == 0) {
@@ -1100,55 +1108,67 @@ __global__ void __launch_bounds__(kPaThreads, 1) k_pattn(const __grid_constant__
 }
 
 // Joins the states that the items of a row left: o = sum_i 2^(m_i - M) O_i / sum_i 2^(m_i - M) l_i, in split order.
-// One warp per (token, head), lane = 4 (head_dim 128) or 2 dims.
-template <class T, int HD>
-__global__ void __launch_bounds__(256) k_pattn_combine(const __grid_constant__ PaArgs p) {
-    constexpr int V = HD / 32;
+// lane = row, warp = 4 DV of the dims, so the states are read in whole lines, several splits' at a time.  It starts while
+// the items still run (programmatic launch) and finds its rows' requests meanwhile.  DV = 4 reads each (max, sum) least
+// often; with few rows DV = 1 gives the SMs four times the warps (1024 rows of 23 splits: 36 -> @C1@ us).
+constexpr int kPaJoinWarps = 4;
+template <class T, int HD, int DV>
+__global__ void __launch_bounds__(kPaJoinWarps * 32) k_pattn_combine(const __grid_constant__ PaArgs p) {
+    constexpr int U = DV == 1 ? 8 : 4;
     const sd_attn_args& a = p.a;
-    const int tok = blockIdx.x, head = blockIdx.y * 8 + (threadIdx.x >> 5), lane = threadIdx.x & 31;
-    if (head >= a.n_heads) return;
+    const int lane = threadIdx.x & 31, d0 = (blockIdx.y * kPaJoinWarps + (threadIdx.x >> 5)) * 4 * DV;
+    const size_t ld = (size_t)a.n_tokens * a.n_heads, row = (size_t)blockIdx.x * 32 + lane;
+    const int gt = (int)min(row, ld - 1) / p.G, tok = gt % a.n_tokens, kvh = gt / a.n_tokens;
+    const int head = kvh * p.G + (int)(row - (size_t)gt * p.G);
     const int b = pa_request(a, tok), t = tok - a.q_start[b], rows = pa_rows(a, b);
-    if (t < 0 || t >= rows) return;
     const int kv = pa_kv(a, b);
     const bool inl = pa_inline(p, rows);
     int size;
     const int chunks = pa_chunks(p, kv, inl, &size);
-    if (chunks == 1 && (a.prefix_len == 0 || inl)) return;  // written by its item
-    const bool seeing = kv - pa_q(a, b) + t >= 0;
+    // else: no row, or written by its item
+    const bool mine = row < ld && t >= 0 && t < rows && !(chunks == 1 && (a.prefix_len == 0 || inl));
+    const bool seeing = mine && kv - pa_q(a, b) + t >= 0;
     const int s0 = inl ? p.cp : 0, s1 = seeing ? p.cp + chunks : s0;
-    const size_t row = (size_t)tok * a.n_heads + head, ld = (size_t)a.n_tokens * a.n_heads;
+    pdl_wait();
+    if (!__any_sync(0xffffffffu, mine)) return;
     float M = -INFINITY;
-    for (int s = s0 + lane; s < s1; s += 32) M = fmaxf(M, p.ml[s * ld + row].x);
-    M = warp_max(M);
+#pragma unroll 8
+    for (int s = s0; s < s1; ++s) M = fmaxf(M, p.ml[s * ld + row].x);
     if (M == -INFINITY) M = 0.f;
-    float L = 0.f, o[V];
+    float L = 0.f;
+    float4 o[DV];
 #pragma unroll
-    for (int e = 0; e < V; ++e) o[e] = 0.f;
-    for (int c = s0; c < s1; c += 32) {
-        // lane l: weight of split c + l (0 where it saw nothing, and its O is then not defined)
-        const float2 ml = c + lane < s1 ? p.ml[(c + lane) * ld + row] : make_float2(0.f, 0.f);
-        const float f = ml.y == 0.f ? 0.f : ex2(ml.x - M);
-        L = fmaf(ml.y, f, L);
-        for (int s = c; s < min(s1, c + 32); s += 8) {  // eight splits' O in flight
-            float acc[8][V];
+    for (int e = 0; e < DV; ++e) o[e] = make_float4(0.f, 0.f, 0.f, 0.f);
+    const float4* acc = p.acc + (size_t)(d0 / 4) * ld + row;
+    for (int c = s0; c < s1; c += U) {
+        float2 ml[U];
+        float4 x[U][DV];
 #pragma unroll
-            for (int u = 0; u < 8; ++u) {
-                const float fu = __shfl_sync(0xffffffffu, f, (s - c + u) & 31);
-                const float* src = p.acc + ((s + u) * ld + row) * HD + lane * V;
+        for (int u = 0; u < U; ++u) {
+            const int s = min(c + u, s1 - 1);
+            ml[u] = p.ml[s * ld + row];
 #pragma unroll
-                for (int e = 0; e < V; ++e) acc[u][e] = s + u < s1 && fu != 0.f ? src[e] * fu : 0.f;
+            for (int e = 0; e < DV; ++e) x[u][e] = acc[((size_t)s * (HD / 4) + e) * ld];
+        }
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            if (c + u >= s1 || ml[u].y == 0.f) continue;  // a split that saw nothing has no O
+            const float f = ex2(ml[u].x - M);
+            L = fmaf(ml[u].y, f, L);
+#pragma unroll
+            for (int e = 0; e < DV; ++e) {
+                o[e].x = fmaf(x[u][e].x, f, o[e].x);
+                o[e].y = fmaf(x[u][e].y, f, o[e].y);
+                o[e].z = fmaf(x[u][e].z, f, o[e].z);
+                o[e].w = fmaf(x[u][e].w, f, o[e].w);
             }
-#pragma unroll
-            for (int u = 0; u < 8; ++u)
-#pragma unroll
-                for (int e = 0; e < V; ++e) o[e] += acc[u][e];
         }
     }
-    L = warp_sum(L);
+    if (!mine) return;
     const float inv = L > 0.f ? 1.f / L : (L == 0.f ? 0.f : L);
-    uint32_t* dst = reinterpret_cast<uint32_t*>(static_cast<T*>(a.out) + (size_t)tok * a.out_ld + (size_t)head * a.out_head + lane * V);
+    uint2* dst = reinterpret_cast<uint2*>(static_cast<T*>(a.out) + (size_t)tok * a.out_ld + (size_t)head * a.out_head + d0);
 #pragma unroll
-    for (int e = 0; e < V / 2; ++e) dst[e] = pa_pack<T>(o[2 * e] * inv, o[2 * e + 1] * inv);
+    for (int e = 0; e < DV; ++e) dst[e] = make_uint2(pa_pack<T>(o[e].x * inv, o[e].y * inv), pa_pack<T>(o[e].z * inv, o[e].w * inv));
 }
 
 // ---------------------------------------------------------------------------------------------
@@ -1257,21 +1277,33 @@ int launch_tc(const PaArgs& p, int grid, int dev, cudaStream_t st) {
     k_pattn<T, HD, MOD><<<grid, kPaThreads, smem, st>>>(p);
     if ((e = cudaGetLastError()) != cudaSuccess) return cuda_fail(e, "attention");
     if (pa_splits(p) > 0) {
-        k_pattn_combine<T, HD><<<dim3(p.a.n_tokens, (p.a.n_heads + 7) / 8), 256, 0, st>>>(p);
-        if ((e = cudaGetLastError()) != cudaSuccess) return cuda_fail(e, "attention combine");
+        cudaLaunchConfig_t cfg{};
+        const unsigned blocks = (unsigned)(((long long)p.a.n_tokens * p.a.n_heads + 31) / 32);
+        const bool many = blocks >= (unsigned)device_sm_count(dev);
+        cfg.gridDim = dim3(blocks, HD / 4 / kPaJoinWarps / (many ? 4 : 1));
+        cfg.blockDim = dim3(kPaJoinWarps * 32);
+        cfg.stream = st;
+        cudaLaunchAttribute at{};
+        at.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+        at.val.programmaticStreamSerializationAllowed = 1;
+        cfg.attrs = &at;
+        cfg.numAttrs = 1;
+        e = many ? cudaLaunchKernelEx(&cfg, k_pattn_combine<T, HD, 4>, p) : cudaLaunchKernelEx(&cfg, k_pattn_combine<T, HD, 1>, p);
+        if (e != cudaSuccess) return cuda_fail(e, "attention combine");
     }
     return SD_OK;
 }
 
 int run_tc(const sd_attn_args& a, int dev, int* err, cudaStream_t st) {
+    if ((long long)a.n_tokens * a.n_heads > INT32_MAX - 64) return fail(SD_ERR_INVALID, "sd_attention_dev: too many rows");
     PaArgs p{};
     pa_plan(a, device_sm_count(dev), &p);
     const size_t need = pa_workspace(p);
     if (need > 0 && (!a.workspace || a.workspace_bytes < need || (reinterpret_cast<uintptr_t>(a.workspace) & 255)))
         return fail(SD_ERR_INVALID, "sd_attention_dev: %zu bytes of 256-byte aligned workspace needed", need);
     const size_t rows = (size_t)pa_splits(p) * a.n_tokens * a.n_heads;
-    p.acc = static_cast<float*>(a.workspace);
-    p.ml = reinterpret_cast<float2*>(p.acc + rows * a.pool.head_dim);
+    p.acc = static_cast<float4*>(a.workspace);
+    p.ml = reinterpret_cast<float2*>(p.acc + rows * (a.pool.head_dim / 4));
     p.err = err;
     const sd_kv_pool& k = a.pool;
     const bool bf = k.dtype == SD_BF16;
