@@ -221,7 +221,7 @@ __global__ void k_pages_reset(sd_pages p) {
 // ---------------------------------------------------------------------------------------------
 // K/V append: a cast copy, bound by HBM (source read once, pool rows written once).  One warp per token, so its slot is
 // read once; where pointers and strides allow it, lanes move 8 elements at a time and the row's loads are all in flight
-// before the first store.  16384 tokens of 2 x 1024 bf16: @APPEND@
+// before the first store.  16384 tokens of 2 x 1024 bf16: 24.6 us, 5.5 TB/s (110 us with one element per lane).
 // ---------------------------------------------------------------------------------------------
 struct AppendArgs {
     const void *k, *v;

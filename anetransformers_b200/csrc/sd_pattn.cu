@@ -133,6 +133,7 @@ struct PaArgs {
     int np;                // key tiles of the prefix
     int n_pt, cp, ct_pre;  // prefix items: row-tile pairs over the tokens, chunks, tiles per chunk
     int ct_own;            // tiles per chunk of own items
+    bool few;              // own items by k_pattn_rows
     // States of rows whose keys lie in several items, by split; row (kv head, token, head of its group), so that the rows
     // of a tile, one per thread, are neighbours: O as float4 [splits][hd / 4][rows], (max, sum) as [splits][rows].
     float4* acc;
@@ -187,7 +188,7 @@ __device__ __forceinline__ int pa_tiles(const PaArgs& p, int rows) {
 __device__ __forceinline__ int pa_chunks(const PaArgs& p, int kv, bool inl, int* size) {
     const int t = (kv + kPaKeys - 1) / kPaKeys + (inl ? p.np : 0);
     const int n = max(1, (t + p.ct_own - 1) / p.ct_own);
-    *size = p.a.window > 0 ? p.ct_own : (t + n - 1) / n;
+    *size = p.a.window > 0 || p.few ? p.ct_own : (t + n - 1) / n;
     return n;
 }
 __device__ __forceinline__ int pa_request(const sd_attn_args& a, int tok) {
@@ -519,9 +520,9 @@ __global__ void __launch_bounds__(kPaThreads, 1) k_pattn(const __grid_constant__
         bool bad = false;
         for (int b = b0; b < b1; ++b) {
             int size;
-            const int rows = pa_rows(a, b), u = rows > 0 ? pa_tiles(p, rows) * pa_chunks(p, pa_kv(a, b), pa_inline(p, rows), &size) : 0;
-            bad |= a.q_len[b] > a.max_q || a.q_len[b] < 0 || a.kv_len[b] > a.max_kv || a.kv_len[b] < 0 || a.q_start[b] < 0 ||
-                   rows < pa_q(a, b);
+            const int rows = pa_rows(a, b), u = rows > 0 && !p.few ? pa_tiles(p, rows) * pa_chunks(p, pa_kv(a, b), pa_inline(p, rows), &size) : 0;
+            bad |= !p.few && (a.q_len[b] > a.max_q || a.q_len[b] < 0 || a.kv_len[b] > a.max_kv || a.kv_len[b] < 0 || a.q_start[b] < 0 ||
+                   rows < pa_q(a, b));
             ustart[b] = u;
             sum += u;
         }
@@ -1107,10 +1108,306 @@ __global__ void __launch_bounds__(kPaThreads, 1) k_pattn(const __grid_constant__
     if (warp == 9) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, 512;" ::"r"(tmem) : "memory");
 }
 
+// ---------------------------------------------------------------------------------------------
+// Few rows: every request of the call has at most 16 query rows per kv head (decode, short verifies).  Reading the
+// request's own K/V bounds it, so the small MMAs of mma.sync do, three CTAs share an SM and hide each other's latencies,
+// and 16-byte asynchronous copies fetch a page of any size equally well (a TMA box of 16 rows is dear, see k_pattn).
+// 64 contexts of 4096, 32 / 8 heads of 128, pages of 16: 8 rows 188 us (5.7 TB/s), 16 rows 204 us against 271 us by
+// k_pattn (203 against 204 with pages of 128); at 20 rows it would take 306 us against 274, so 16 is the limit.  Two stages
+// of 64 keys and three CTAs took 193 us at 64 ragged contexts up to 8192, three stages and two CTAs 235 us.
+//
+// A CTA has one (kv head, chunk, request); four warps take 16 of each 64 keys.  S^T = K Q^T (keys x rows) and
+// O^T = V^T P^T (dims x rows), rows in NT tiles of 8, so nothing is padded to 128 rows; each warp keeps its own running
+// (max, sum, O), joined at the end.  Keys that no row sees are fetched as zeros.
+// ---------------------------------------------------------------------------------------------
+constexpr int kRwThreads = 128, kRwKeys = 64, kRwStages = 2, kRwMaxRows = 16;
+template <int HD> constexpr int rw_ld() { return HD + 8; }  // padded row of shared memory: ldmatrix without conflicts
+template <int HD, int NT>
+constexpr size_t rw_smem() {
+    return ((size_t)NT * 8 + kRwStages * 2 * kRwKeys) * rw_ld<HD>() * 2;
+}
+
+__device__ __forceinline__ void rw_cp16(uint32_t dst, const void* src, bool ok) {
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(ok ? 16u : 0u) : "memory");
+}
+__device__ __forceinline__ void rw_ldsm2(uint32_t a, uint32_t& x, uint32_t& y) {
+    asm volatile("ldmatrix.sync.aligned.m8n8.x2.shared.b16 {%0, %1}, [%2];" : "=r"(x), "=r"(y) : "r"(a) : "memory");
+}
+__device__ __forceinline__ void rw_ldsm4(uint32_t a, uint32_t (&r)[4]) {
+    asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0, %1, %2, %3}, [%4];"
+                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+                 : "r"(a)
+                 : "memory");
+}
+__device__ __forceinline__ void rw_ldsm4t(uint32_t a, uint32_t (&r)[4]) {
+    asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0, %1, %2, %3}, [%4];"
+                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+                 : "r"(a)
+                 : "memory");
+}
+__device__ __forceinline__ uint32_t rw_transpose(uint32_t x) {
+    uint32_t y;
+    asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
+    return y;
+}
+template <class T>
+__device__ __forceinline__ void rw_mma(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+    if constexpr (std::is_same<T, __half>::value)
+        asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+                     : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+                     : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+    else
+        asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+                     : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+                     : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+
+template <class T, int HD, int NT>
+__global__ void __launch_bounds__(kRwThreads) k_pattn_rows(const __grid_constant__ PaArgs p) {
+    constexpr bool BF = !std::is_same<T, __half>::value;
+    constexpr float kShift = BF ? 0.f : 6.f, kSlack = 8.f;  // as in k_pattn
+    constexpr int LD = rw_ld<HD>(), CPR = HD / 8, KPP = kRwThreads / CPR;  // 16-byte pieces per row, keys per pass
+    extern __shared__ __align__(16) uint8_t rsm[];
+    const sd_attn_args& a = p.a;
+    const int kvh = blockIdx.x, c = blockIdx.y, b = blockIdx.z, tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    const int n_tok = pa_rows(a, b), q = pa_q(a, b), kv = pa_kv(a, b), G = p.G, W = a.window;
+    if (kvh == 0 && c == 0 && tid == 0 &&
+        (a.q_len[b] > a.max_q || a.q_len[b] < 0 || a.kv_len[b] > a.max_kv || a.kv_len[b] < 0 || a.q_start[b] < 0 || n_tok < q))
+        set_dev_error(p.err, DEV_ERR_BAD_ARG);
+    pdl_trigger();
+    if (n_tok == 0) return;
+    int size;
+    const int chunks = pa_chunks(p, kv, false, &size);
+    if (c >= chunks) return;
+    const int q0 = max(a.q_start[b], 0), base = kv - q, nrow = n_tok * G;
+    const int hi = min(max(base + n_tok, 0), min(kv, (c + 1) * size * kPaKeys)), lo = W > 0 ? max(0, base + 1 - W) : 0;
+    const int first = max(c * size * kPaKeys, lo & ~(kRwKeys - 1));
+    const int n = first < hi ? (hi - first + kRwKeys - 1) / kRwKeys : 0;
+    T* qsm = reinterpret_cast<T*>(rsm);
+    T* ring = qsm + NT * 8 * LD;
+    const int ps = a.pool.page_size, lps = 31 - __clz(ps);
+    const int32_t* table = a.table + (size_t)b * a.table_ld;
+
+    // this thread's pieces of a stage: elements d8.. of keys key0 + KPP i
+    const int d8 = (tid % CPR) * 8, key0 = tid / CPR;
+    const T* kp = static_cast<const T*>(a.pool.k) + (size_t)kvh * a.pool.head_stride + d8;
+    const T* vp = static_cast<const T*>(a.pool.v) + (size_t)kvh * a.pool.head_stride + d8;
+    int ids[4];  // pages of the next stage's 16-key groups
+    auto load_ids = [&](int s) {
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            const int k = first + s * kRwKeys + 16 * j;
+            ids[j] = s < n && k < hi && k + 16 > lo ? table[k >> lps] : -2;
+        }
+    };
+    uint32_t masks = 0;  // 4 bits per stage: groups that are there; the latest issued lowest
+    auto issue = [&](int s) {
+        if (s < n) {
+            uint32_t m = 0;
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                const bool have = ids[j] >= 0 && ids[j] < a.pool.n_pages;
+                if (!have && ids[j] != -2 && tid == 0) set_dev_error(p.err, DEV_ERR_BAD_ARG);
+                m |= (uint32_t)have << j;
+            }
+            masks = masks << 4 | m;
+            const uint32_t dst = smem_u32(ring + (size_t)(s % kRwStages) * 2 * kRwKeys * LD + key0 * LD + d8);
+#pragma unroll
+            for (int i = 0; i < kRwKeys / KPP; ++i) {
+                const int r = key0 + i * KPP, k = first + s * kRwKeys + r, j = (i * KPP) >> 4;
+                // KPP <= 16 divides 16: a pass lies in one group
+                const bool ok = (m >> j & 1) && k < hi && k >= lo;
+                const size_t at = ok ? (size_t)ids[j] * a.pool.page_stride + (size_t)(k & (ps - 1)) * a.pool.pos_stride : 0;
+                rw_cp16(dst + i * KPP * LD * 2, kp + at, ok);
+                rw_cp16(dst + (kRwKeys + i * KPP) * LD * 2, vp + at, ok);
+            }
+        } else {
+            masks <<= 4;
+        }
+        asm volatile("cp.async.commit_group;" ::: "memory");
+    };
+    load_ids(0);
+#pragma unroll
+    for (int s = 0; s < kRwStages - 1; ++s) {
+        issue(s);
+        load_ids(s + 1);
+    }
+    // Q rows (token, head of the group), zero behind them
+    for (int i = tid; i < NT * 8 * CPR; i += kRwThreads) {
+        const int r = i / CPR, d = (i - r * CPR) * 8;
+        uint4 x = make_uint4(0, 0, 0, 0);
+        if (r < nrow) {
+            const int t = r / G, h = r - t * G;
+            x = *reinterpret_cast<const uint4*>(static_cast<const T*>(a.q) + (size_t)(q0 + t) * a.q_ld + (size_t)(kvh * G + h) * a.q_head + d);
+        }
+        *reinterpret_cast<uint4*>(qsm + r * LD + d) = x;
+    }
+    // the rows whose scores this thread holds: 8 nt + 2 (lane % 4) + e
+    const int g = lane >> 2, t4 = lane & 3, lr = lane & 7, lq = lane >> 3;
+    int end[NT][2];  // first key that the row does not see
+    float slope[NT][2];
+    const float kLog2e = 1.4426950408889634f, sc2 = a.scale * kLog2e;
+    const float cap2 = a.softcap * kLog2e, x1 = a.softcap > 0.f ? a.scale / a.softcap : 0.f;
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+            const int r = nt * 8 + 2 * t4 + e, t = r / G;
+            end[nt][e] = r < nrow ? max(base + t + 1, 0) : 0;
+            slope[nt][e] = a.alibi && r < nrow ? a.alibi[kvh * G + r - t * G] * kLog2e : 0.f;
+        }
+    float m[NT][2], l[NT][2], o[HD / 16][NT][4];
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+        for (int e = 0; e < 2; ++e) m[nt][e] = -INFINITY, l[nt][e] = 0.f;
+#pragma unroll
+    for (int i = 0; i < HD / 16; ++i)
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) o[i][nt][e] = 0.f;
+    const uint32_t q_a = smem_u32(qsm + lr * LD + (lq & 1) * 8);
+    const uint32_t k_off = ((warp * 16 + lr + (lq & 1) * 8) * LD + (lq >> 1) * 8) * 2;
+    const uint32_t v_off = ((kRwKeys + warp * 16 + lr + (lq >> 1) * 8) * LD + (lq & 1) * 8) * 2;
+    for (int s = 0; s < n; ++s) {
+        asm volatile("cp.async.wait_group %0;" ::"n"(kRwStages - 2) : "memory");
+        __syncthreads();  // stage s is there for everyone; the one before it is free
+        issue(s + kRwStages - 1);
+        load_ids(s + kRwStages);
+        const uint32_t st = smem_u32(ring + (size_t)(s % kRwStages) * 2 * kRwKeys * LD);
+        float sc[NT][4];
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt) sc[nt][0] = sc[nt][1] = sc[nt][2] = sc[nt][3] = 0.f;
+#pragma unroll
+        for (int ks = 0; ks < HD / 16; ++ks) {
+            uint32_t kf[4];
+            rw_ldsm4(st + k_off + ks * 32, kf);
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt) {
+                uint32_t b0, b1;
+                rw_ldsm2(q_a + (nt * 8 * LD + ks * 16) * 2, b0, b1);
+                rw_mma<T>(sc[nt], kf, b0, b1);
+            }
+        }
+        const int kg = first + s * kRwKeys + warp * 16 + g;  // this thread's keys: kg and kg + 8
+        const bool there = masks >> (4 * (kRwStages - 1) + warp) & 1;
+        uint32_t pf[NT][2];
+        float fac[NT][2];
+        bool rise = false;
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt) {
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                const int k = kg + (e >> 1) * 8, stop = end[nt][e & 1];
+                float z;
+                if (a.softcap > 0.f) {
+                    const float x = sc[nt][e] * x1;
+                    z = fmaf(rcp(1.f + ex2(x * (2.f * kLog2e))), -2.f * cap2, cap2);
+                } else {
+                    z = sc[nt][e] * sc2;
+                }
+                if (a.alibi) z = fmaf(slope[nt][e & 1], (float)(k - (stop - 1)), z);
+                if (!there || k >= stop || (W > 0 && k < stop - W)) z = -INFINITY;
+                sc[nt][e] = z;
+            }
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+                float top = fmaxf(sc[nt][e], sc[nt][e + 2]);
+#pragma unroll
+                for (int off = 4; off < 32; off <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, off));
+                fac[nt][e] = 1.f;
+                if (top > m[nt][e] + kSlack || (m[nt][e] == -INFINITY && top != -INFINITY)) {
+                    fac[nt][e] = ex2(m[nt][e] - top);
+                    m[nt][e] = top;
+                    rise = true;
+                }
+                const float ref = (m[nt][e] == -INFINITY ? 0.f : m[nt][e]) - kShift;
+                sc[nt][e] = ex2(sc[nt][e] - ref);
+                sc[nt][e + 2] = ex2(sc[nt][e + 2] - ref);
+                l[nt][e] = fmaf(l[nt][e], fac[nt][e], sc[nt][e] + sc[nt][e + 2]);
+            }
+            pf[nt][0] = rw_transpose(pa_pack<T>(sc[nt][0], sc[nt][1]));
+            pf[nt][1] = rw_transpose(pa_pack<T>(sc[nt][2], sc[nt][3]));
+        }
+        if (__any_sync(0xffffffffu, rise)) {
+#pragma unroll
+            for (int i = 0; i < HD / 16; ++i)
+#pragma unroll
+                for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) o[i][nt][e] *= fac[nt][e & 1];
+        }
+#pragma unroll
+        for (int i = 0; i < HD / 16; ++i) {
+            uint32_t vf[4];
+            rw_ldsm4t(st + v_off + i * 32, vf);
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt) rw_mma<T>(o[i][nt], vf, pf[nt][0], pf[nt][1]);
+        }
+    }
+    asm volatile("cp.async.wait_all;" ::: "memory");
+    __syncthreads();  // the ring becomes the warps' states: O [warp][row][dim], (max, sum) [warp][row]
+    constexpr int OLD = HD + 4;
+    float* osm = reinterpret_cast<float*>(ring);
+    float2* msm = reinterpret_cast<float2*>(osm + 4 * NT * 8 * OLD);
+    static_assert((size_t)4 * NT * 8 * (OLD * 4 + 8) <= (size_t)kRwStages * 2 * kRwKeys * LD * 2, "the states fit the ring");
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt) {
+#pragma unroll
+        for (int e = 0; e < 2; ++e)
+#pragma unroll
+            for (int off = 4; off < 32; off <<= 1) l[nt][e] += __shfl_xor_sync(0xffffffffu, l[nt][e], off);
+#pragma unroll
+        for (int i = 0; i < HD / 16; ++i)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) osm[(warp * NT * 8 + nt * 8 + 2 * t4 + (e & 1)) * OLD + i * 16 + g + (e >> 1) * 8] = o[i][nt][e];
+        if (g == 0) {
+            msm[warp * NT * 8 + nt * 8 + 2 * t4] = make_float2(m[nt][0], l[nt][0]);
+            msm[warp * NT * 8 + nt * 8 + 2 * t4 + 1] = make_float2(m[nt][1], l[nt][1]);
+        }
+    }
+    __syncthreads();
+    const bool direct = chunks == 1 && a.prefix_len == 0;
+    const size_t ld = (size_t)a.n_tokens * a.n_heads;
+    for (int i = tid; i < nrow * (HD / 4); i += kRwThreads) {
+        // neighbouring threads: neighbouring rows of the workspace, or neighbouring dims of the output
+        const int r = direct ? i / (HD / 4) : i % nrow, d4 = direct ? i % (HD / 4) : i / nrow;
+        float M = -INFINITY, L = 0.f;
+        float2 ml[4];
+#pragma unroll
+        for (int w = 0; w < 4; ++w) {
+            ml[w] = msm[w * NT * 8 + r];
+            M = fmaxf(M, ml[w].x);
+        }
+        float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+        for (int w = 0; w < 4; ++w) {
+            const float f = ml[w].x == -INFINITY && ml[w].y == 0.f ? 0.f : ex2(ml[w].x - M);
+            const float4 y = *reinterpret_cast<const float4*>(osm + (w * NT * 8 + r) * OLD + d4 * 4);
+            L = fmaf(ml[w].y, f, L);
+            x.x = fmaf(y.x, f, x.x);
+            x.y = fmaf(y.y, f, x.y);
+            x.z = fmaf(y.z, f, x.z);
+            x.w = fmaf(y.w, f, x.w);
+        }
+        const int t = r / G, h = r - t * G;
+        if (direct) {
+            const float inv = L > 0.f ? 1.f / L : (L == 0.f ? 0.f : L);
+            T* dst = static_cast<T*>(a.out) + (size_t)(q0 + t) * a.out_ld + (size_t)(kvh * G + h) * a.out_head + d4 * 4;
+            *reinterpret_cast<uint2*>(dst) = make_uint2(pa_pack<T>(x.x * inv, x.y * inv), pa_pack<T>(x.z * inv, x.w * inv));
+        } else {
+            const size_t prow = ((size_t)kvh * a.n_tokens + q0 + t) * G + h;
+            p.acc[((size_t)(p.cp + c) * (HD / 4) + d4) * ld + prow] = x;
+            if (d4 == 0) p.ml[(size_t)(p.cp + c) * ld + prow] = make_float2(M, L);
+        }
+    }
+}
+
 // Joins the states that the items of a row left: o = sum_i 2^(m_i - M) O_i / sum_i 2^(m_i - M) l_i, in split order.
 // lane = row, warp = 4 DV of the dims, so the states are read in whole lines, several splits' at a time.  It starts while
 // the items still run (programmatic launch) and finds its rows' requests meanwhile.  DV = 4 reads each (max, sum) least
-// often; with few rows DV = 1 gives the SMs four times the warps (1024 rows of 23 splits: 36 -> @C1@ us).
+// often; with few rows DV = 1 gives the SMs four times the warps (1024 rows of 23 splits: 36 -> 11 us).
 constexpr int kPaJoinWarps = 4;
 template <class T, int HD, int DV>
 __global__ void __launch_bounds__(kPaJoinWarps * 32) k_pattn_combine(const __grid_constant__ PaArgs p) {
@@ -1212,7 +1509,11 @@ void pa_plan(const sd_attn_args& a, int sms, PaArgs* p) {
     // tiles that an item can see through the window; if those fit one chunk, nothing is cut
     const int seen = a.window > 0 ? (int)std::min<long long>(own, ((long long)a.window + std::min(a.max_q, pair)) / kPaKeys + 2) : own;
     int ct = std::max(seen, 1);
-    if (a.max_q <= p->TPT) {
+    p->few = (long long)a.max_q * p->G <= kRwMaxRows;
+    if (p->few) {
+        // a chunk costs about a tile to start and to join; the kernel keeps several CTAs on an SM
+        ct = std::max(1, (int)(std::sqrt((double)units * seen / (2.0 * sms)) + 0.5));
+    } else if (a.max_q <= p->TPT) {
         // few rows per item: a chunk costs about one tile to start and to join, and the last one to end leaves the
         // other SMs idle for up to its length: the sum is least at the square root of an SM's tiles
         const double per_sm = (double)units * seen / sms;
@@ -1264,6 +1565,23 @@ int encode(CUtensorMap* m, bool bf16, int rank, const void* base, const cuuint64
 
 static_assert(pa_smem<128>(SD_PAGES_MAX_REQ) <= 232448, "the largest batch fits the shared memory");
 
+template <class T, int HD, int NT>
+int launch_rows(const PaArgs& p, int dev, cudaStream_t st) {
+    static std::atomic<bool> ready[64];
+    cudaError_t e = cudaSuccess;
+    if (dev < 0 || dev >= 64 || !ready[dev].load(std::memory_order_acquire)) {
+        e = cudaFuncSetAttribute(k_pattn_rows<T, HD, NT>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)rw_smem<HD, NT>());
+        if (e != cudaSuccess) return cuda_fail(e, "attention attributes");
+        if (dev >= 0 && dev < 64) ready[dev].store(true, std::memory_order_release);
+    }
+    const int own = (p.a.max_kv + kPaKeys - 1) / kPaKeys;
+    const int chunks = std::max(1, (own + p.ct_own - 1) / p.ct_own);
+    if (chunks > 65535) return fail(SD_ERR_INVALID, "sd_attention_dev: too many work items");
+    k_pattn_rows<T, HD, NT><<<dim3(p.a.pool.n_kv_heads, chunks, p.a.n_req), kRwThreads, rw_smem<HD, NT>(), st>>>(p);
+    e = cudaGetLastError();
+    return e == cudaSuccess ? SD_OK : cuda_fail(e, "attention");
+}
+
 template <class T, int HD, bool MOD>
 int launch_tc(const PaArgs& p, int grid, int dev, cudaStream_t st) {
     const size_t smem = pa_smem<HD>(p.a.n_req);
@@ -1274,8 +1592,14 @@ int launch_tc(const PaArgs& p, int grid, int dev, cudaStream_t st) {
         if (e != cudaSuccess) return cuda_fail(e, "attention attributes");
         if (dev >= 0 && dev < 64) ready[dev].store(true, std::memory_order_release);
     }
-    k_pattn<T, HD, MOD><<<grid, kPaThreads, smem, st>>>(p);
-    if ((e = cudaGetLastError()) != cudaSuccess) return cuda_fail(e, "attention");
+    if (grid > 0) {
+        k_pattn<T, HD, MOD><<<grid, kPaThreads, smem, st>>>(p);
+        if ((e = cudaGetLastError()) != cudaSuccess) return cuda_fail(e, "attention");
+    }
+    if (p.few) {
+        const int rc = p.a.max_q * p.G <= 8 ? launch_rows<T, HD, 1>(p, dev, st) : launch_rows<T, HD, 2>(p, dev, st);
+        if (rc) return rc;
+    }
     if (pa_splits(p) > 0) {
         cudaLaunchConfig_t cfg{};
         const unsigned blocks = (unsigned)(((long long)p.a.n_tokens * p.a.n_heads + 31) / 32);
@@ -1325,7 +1649,7 @@ int run_tc(const sd_attn_args& a, int dev, int* err, cudaStream_t st) {
     }
     const int pair = 2 * p.TPT;
     const int own = (a.max_kv + kPaKeys - 1) / kPaKeys + (p.np && a.max_q > pair ? p.np : 0);
-    const long long items = (long long)k.n_kv_heads * ((long long)p.cp * p.n_pt + ((long long)a.n_req + a.n_tokens / pair) *
+    const long long items = (long long)k.n_kv_heads * ((long long)p.cp * p.n_pt + (p.few ? 0LL : (long long)a.n_req + a.n_tokens / pair) *
                                                        std::max(1, (own + p.ct_own - 1) / p.ct_own));
     if (items > INT32_MAX) return fail(SD_ERR_INVALID, "sd_attention_dev: too many work items");
     const int grid = (int)items;
