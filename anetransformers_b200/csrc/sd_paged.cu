@@ -66,7 +66,8 @@ namespace {
 // cluster.  Every CTA of the cluster computes the sums for itself (cheaper than handing them over), then the
 // scatters are dealt over the cluster's threads, each finding its request by bisection in shared memory.  Cluster
 // barriers separate reading the old state, pushing, taking and reading the new table; a step that moves no page
-// passes none.
+// passes none.  One request and token: 3.6 us; 256 requests, 1280 tokens: 9.3 us (23 us by one CTA); 64 prompts replaced
+// by 64 others, 36 thousand tokens: 15 us (59 us by one CTA).
 // ---------------------------------------------------------------------------------------------
 constexpr int kPlanThreads = 512;
 
@@ -157,18 +158,44 @@ __global__ void __launch_bounds__(kPlanThreads) k_pages_plan(const PlanArgs a) {
     const int count = min(count0 + n_back, a.n_pages), left = max(count - n_want, 0);
     if (n_back | n_want) {
         cluster.sync();  // every CTA has read the old state
-        for (int k = gtid; k < n_back; k += gn) {
-            const int b = owner(back, n, k);
-            const size_t i = (size_t)b * a.table_ld + base[b] + (k - back[b]);
-            if (count0 + k < a.n_pages) a.free_pages[count0 + k] = a.table[i];
-            a.table[i] = -1;
+        for (int k0 = gtid; k0 < n_back; k0 += 4 * gn) {
+            size_t i[4];
+            int page[4];
+#pragma unroll
+            for (int u = 0; u < 4; ++u) {
+                const int k = k0 + u * gn;
+                if (k >= n_back) continue;
+                const int b = owner(back, n, k);
+                i[u] = (size_t)b * a.table_ld + base[b] + (k - back[b]);
+                page[u] = a.table[i[u]];
+            }
+#pragma unroll
+            for (int u = 0; u < 4; ++u) {
+                const int k = k0 + u * gn;
+                if (k >= n_back) continue;
+                if (count0 + k < a.n_pages) a.free_pages[count0 + k] = page[u];
+                a.table[i[u]] = -1;
+            }
         }
         if (n_back && n_want) cluster.sync();  // what was given back can be taken
-        for (int k = gtid; k < n_want; k += gn) {
-            if (k >= count) break;
-            const int b = owner(want, n, k);
-            a.table[(size_t)b * a.table_ld + base[b] + (k - want[b])] = a.free_pages[count - 1 - k];
-            a.free_pages[count - 1 - k] = -1;
+        for (int k0 = gtid; k0 < min(n_want, count); k0 += 4 * gn) {
+            size_t i[4];
+            int page[4];
+#pragma unroll
+            for (int u = 0; u < 4; ++u) {
+                const int k = k0 + u * gn;
+                if (k >= n_want || k >= count) continue;
+                page[u] = a.free_pages[count - 1 - k];
+                const int b = owner(want, n, k);
+                i[u] = (size_t)b * a.table_ld + base[b] + (k - want[b]);
+            }
+#pragma unroll
+            for (int u = 0; u < 4; ++u) {
+                const int k = k0 + u * gn;
+                if (k >= n_want || k >= count) continue;
+                a.table[i[u]] = page[u];
+                a.free_pages[count - 1 - k] = -1;
+            }
         }
         for (int b = gtid; b < n; b += gn) {
             const int w = want[b + 1] - want[b];
@@ -321,7 +348,8 @@ int launch_pages_plan(const sd_pages* p, const int32_t* kv_len, const int32_t* q
     if (smem > 48 * 1024 - 1024)
         e = cudaFuncSetAttribute(k_pages_plan, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
     if (e != cudaSuccess) return cuda_fail(e, "pages plan");
-    const int items = std::max(n_tokens, p->n_req);
+    // a thread's share of a step is a token or a few pages of a request (the host does not know how many move)
+    const long long items = std::max<long long>(n_tokens, 16LL * p->n_req);
     int ctas = 1;
     while (ctas < 8 && ctas * kPlanThreads < items) ctas *= 2;
     cudaLaunchConfig_t cfg{};
