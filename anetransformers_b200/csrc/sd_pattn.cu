@@ -1491,7 +1491,7 @@ EncodeTiled encode_tiled() {
 bool tc_able(const sd_attn_args& a) {
     const sd_kv_pool& k = a.pool;
     auto al = [](const void* q) { return (reinterpret_cast<uintptr_t>(q) & 15) == 0; };
-    auto st = [](int64_t s) { return s % 8 == 0 && s < (1ll << 38); };
+    auto st = [](int64_t s) { return s > 0 && s % 8 == 0 && s < (1ll << 38); };
     return (k.head_dim == 64 || k.head_dim == 128) && al(k.k) && al(k.v) && al(a.q) && al(a.out) && st(k.page_stride) &&
            st(k.pos_stride) && st(k.head_stride) && st(a.q_ld) && st(a.q_head) && st(a.out_ld) && st(a.out_head);
 }
@@ -1680,7 +1680,7 @@ int check_attention(const sd_attn_args* a) {
                     a->pool.page_size);
     if ((int64_t)a->prefix_len + a->max_kv > INT32_MAX - 1024) return fail(SD_ERR_INVALID, "%s: prefix too long", what);
     if (a->prefix_len > 0 && !a->prefix_table) return fail(SD_ERR_INVALID, "%s: a prefix needs its table", what);
-    if (!(a->softcap >= 0.f) || !(a->scale == a->scale) || a->softcap > 1e30f)
+    if (!(std::fabs(a->scale) <= 1e30f) || !(a->softcap == 0.f || (a->softcap >= 1e-6f && a->softcap <= 1e30f)))
         return fail(SD_ERR_INVALID, "%s: scale %g, softcap %g", what, a->scale, a->softcap);
     if (a->q_head < a->pool.head_dim || a->out_head < a->pool.head_dim || a->q_ld < 0 || a->out_ld < 0)
         return fail(SD_ERR_INVALID, "%s: strides", what);

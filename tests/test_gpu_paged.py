@@ -311,6 +311,66 @@ def test_score_options(pg, opts, prefix):
     check_attention(pg, make_case([300, 140], [300, 100], 8, 2, 128, 16, "bfloat16", prefix=prefix, seed=4), opts)
 
 
+@pytest.mark.parametrize("opts", [dict()] + OPTS, ids=lambda o: "-".join(f"{k}{v}" for k, v in o.items()) or "plain")
+@pytest.mark.parametrize("prefix", [0, 130])
+@pytest.mark.parametrize("q,hd,dtype,page", [(1, 128, "bfloat16", 16), (2, 64, "float16", 32), (3, 128, "float16", 256), (4, 64, "bfloat16", 64)])
+def test_few_rows(pg, q, hd, dtype, page, prefix, opts):
+    """At most 16 rows per kv head (groups of 4 heads, up to 4 tokens): decode and short verifies, lengths around the
+    borders of stages (64 keys), tiles and pages, idle and ended requests, several splits."""
+    import torch
+    opts = dict(opts)
+    if opts.get("alibi"):
+        opts["alibi"] = torch.exp2(-torch.arange(1, 9, dtype=torch.float32)).cuda()
+    kv = [1, 63, 64, 65, 130, 0, 700, 17, 128, 1500]
+    qs = [min(q, max(x, 1)) if i % 3 else min(1, x) for i, x in enumerate(kv)]
+    qs[7] = 0
+    check_attention(pg, make_case(kv, qs, 8, 2, hd, page, dtype, prefix=prefix, seed=q), opts)
+
+
+@pytest.mark.parametrize("heads,hk,q", [(16, 1, 1), (17, 1, 1), (32, 1, 3), (100, 1, 2), (128, 1, 4), (65, 1, 3), (3, 3, 16), (3, 3, 17)])
+def test_group_sizes(pg, heads, hk, q):
+    """Groups from 1 to 128 heads per kv head, on both sides of 16 rows."""
+    check_attention(pg, make_case([40, 200, 3], [q, min(q, 2), min(q, 3)], heads, hk, 64, 16, "bfloat16", prefix=20, seed=heads))
+
+
+@pytest.mark.parametrize("q", [1, 9])
+def test_no_keys_at_all(pg, q):
+    """Every request empty: rows without a position are 0, and nothing is read."""
+    for prefix in (0, 30):
+        got = check_attention(pg, make_case([0, 0], [q, 1], 8, 2, 64, 16, "float16", prefix=prefix, seed=1), max_kv=0)
+        assert not got.any()
+
+
+@pytest.mark.parametrize("q", [2, 70])
+def test_two_calls_at_once(pg, q):
+    """Calls in flight on two streams, each again and again, give what each gives alone."""
+    import torch
+    cases = [make_case([300, 900, 40], [q, 1, 2], 8, 2, 128, 16, "bfloat16", prefix=200, seed=30 + i) for i in range(2)]
+    dev = [{k: (v.cuda() if hasattr(v, "cuda") else v) for k, v in c.items()} for c in cases]
+
+    def call(d):
+        return pg.attention_dev(d["q"], d["k_pages"], d["v_pages"], d["table"], d["kv_len"], d["q_start"], d["q_len"], max_q=q,
+                                max_kv=900, prefix_table=d["prefix_table"], prefix_len=200)
+    want = [call(d) for d in dev]
+    streams = [torch.cuda.Stream() for _ in dev]
+    torch.cuda.synchronize()
+    got = [[], []]
+    for _ in range(20):
+        for i, st in enumerate(streams):
+            with torch.cuda.stream(st):
+                got[i].append(call(dev[i]))
+    torch.cuda.synchronize()
+    for i in range(2):
+        assert all(torch.equal(x, want[i]) for x in got[i])
+
+
+def test_one_query_for_all_tokens(pg):
+    """q with a token stride of 0 (an expanded row)."""
+    c = make_case([50, 90], [3, 1], 4, 2, 64, 16, "float16", seed=31)
+    c["q"] = c["q"][:1].expand(4, -1, -1).clone()
+    check_attention(pg, c, q=c["q"][:1].cuda().expand(4, -1, -1))
+
+
 def test_rows_without_positions(pg):
     """More new tokens than positions: the first rows have no position and are 0; requests of length 0 too."""
     for prefix in (0, 40):

@@ -76,7 +76,7 @@ def test_append_refusals():
                                 dict(n_req=0), dict(n_req=4097), dict(n_heads=0), dict(n_heads=30), dict(n_heads=8 * 129), dict(max_kv=129),
                                 dict(max_q=-1), dict(max_kv=-1), dict(n_tokens=-1), dict(prefix_len=-1), dict(prefix_len=16),
                                 dict(window=-1), dict(table_ld=0), dict(softcap=-1.0), dict(softcap=float("nan")),
-                                dict(scale=float("nan")), dict(q_head=64), dict(out_head=64),
+                                dict(scale=float("nan")), dict(scale=float("inf")), dict(softcap=1e-9), dict(softcap=float("inf")), dict(q_head=64), dict(out_head=64),
                                 dict(prefix_len=(1 << 31) - 600, prefix_table=P)])
 def test_attention_refusals(kw):
     refused(_lib.lib().sd_attention_dev(C.byref(attn(**kw)), None))
