@@ -102,7 +102,6 @@ __global__ void __launch_bounds__(128) k_pattn_general(const sd_attn_args a, int
         if (lane + 32 * i < hd) out[lane + 32 * i] = pa_from<T>(acc[i] * inv);
 }
 
-
 // ---------------------------------------------------------------------------------------------
 // Tensor-core kernel (head_dim 64 and 128): tcgen05.mma with S, P and O in tensor memory, K/V tiles by TMA.
 //
@@ -118,9 +117,18 @@ __global__ void __launch_bounds__(128) k_pattn_general(const sd_attn_args a, int
 // the workspace for k_pattn_combine; others are written by their item.
 //
 // Warps (12): 0-3 softmax of slot 0, 4-7 of slot 1 (thread = row), 8 TMA and the handing out of items, 9 and 11 MMA
-// issue of slot 0 and 1, 10 zeroes V rows that no row may see (0 x NaN is NaN in the product).  P overwrites S in tensor memory and is the A operand of P V.
+// issue of slot 0 and 1, 10 zeroes V rows that no row may see (0 x NaN is NaN in the product).  P overwrites S in
+// tensor memory and is the A operand of P V.
 // The running maximum that O refers to moves only when a row's maximum rises by more than 2^8 (exact: O and the sum
 // refer to the same value), so O is rarely rescaled.  Every wait is bounded in time (sd_common.cuh).
+//
+// What bounds it.  One causal prompt of 9472 tokens, 32 / 8 heads of 128, no bias: 637 us, 1154 TFLOP/s (0.70 of the
+// measured burst rate of a matrix product, 0.83 of the sustained one, which this length of run is nearer to).  256 rows x
+// 128 keys take the tensor cores 2480 clk with S in halves of 64 keys (N = 64, bound by shared memory; 2050 in one
+// piece, but then a slot's softmax and MMAs alternate: 1.4 x slower overall) and the exponentials 2048 clk; each softmax
+// warp needs about 1900 clk per half, of them 500 to 1000 waiting for its share of the exponentials.  Computing part of
+// these on the FMA pipe (every third to eighth pair) changed nothing or cost up to 5 %; 16 softmax warps of half a row
+// each cost 20 %.  With caps and biases the extra arithmetic per score bounds it.
 // ---------------------------------------------------------------------------------------------
 constexpr int kPaThreads = 384;
 constexpr int kPaKeys = 128;        // keys per tile
@@ -520,9 +528,10 @@ __global__ void __launch_bounds__(kPaThreads, 1) k_pattn(const __grid_constant__
         bool bad = false;
         for (int b = b0; b < b1; ++b) {
             int size;
-            const int rows = pa_rows(a, b), u = rows > 0 && !p.few ? pa_tiles(p, rows) * pa_chunks(p, pa_kv(a, b), pa_inline(p, rows), &size) : 0;
-            bad |= !p.few && (a.q_len[b] > a.max_q || a.q_len[b] < 0 || a.kv_len[b] > a.max_kv || a.kv_len[b] < 0 || a.q_start[b] < 0 ||
-                   rows < pa_q(a, b));
+            const int rows = p.few ? 0 : pa_rows(a, b);
+            const int u = rows > 0 ? pa_tiles(p, rows) * pa_chunks(p, pa_kv(a, b), pa_inline(p, rows), &size) : 0;
+            bad |= !p.few && (a.q_len[b] > a.max_q || a.q_len[b] < 0 || a.kv_len[b] > a.max_kv || a.kv_len[b] < 0 ||
+                              a.q_start[b] < 0 || rows < pa_q(a, b));
             ustart[b] = u;
             sum += u;
         }
@@ -552,7 +561,6 @@ __global__ void __launch_bounds__(kPaThreads, 1) k_pattn(const __grid_constant__
     const uint32_t tmem = ctl->tmem;
     const int n_items = (p.cp * p.n_pt + ustart[a.n_req]) * a.pool.n_kv_heads;
     const int ps = a.pool.page_size, G = p.G;
-
 
     if (warp == 8) {
         // ---------------- TMA ----------------
@@ -778,7 +786,10 @@ __global__ void __launch_bounds__(kPaThreads, 1) k_pattn(const __grid_constant__
                 // half by half.  Each 64-key half of a slot's tile is an S buffer of its own: its next S follows its
                 // product at once, while the softmax is at the other half.
                 const int n = it.n, D = it.pair ? 1 : 2, qt = it.pair ? slot : (int)qb;
-                ok = pa_wait(&ctl->qfull[qt], nq[qt] & 1, ctl, p.err, DEV_ERR_FULL_WAIT);
+                // both Q tiles of a pair: a thread that finished ahead of the other must not meet the other's buffer a
+                // phase early in the next item
+                for (int b = it.pair ? 0 : qt; b <= (it.pair ? 1 : qt); ++b)
+                    ok = ok && pa_wait(&ctl->qfull[b], nq[b] & 1, ctl, p.err, DEV_ERR_FULL_WAIT);
                 const uint32_t qa = sw128_lo(qs + qt * TILE, 16);
                 auto mine = [&](int t) { return it.pair || (t & 1) == slot; };
                 auto q_done = [&]() {  // two arrivals: this thread's twice, or each slot's once
