@@ -1530,11 +1530,14 @@ void pa_plan(const sd_attn_args& a, int sms, PaArgs* p) {
         const double per_sm = (double)units * seen / sms;
         ct = std::max(4, (int)(std::sqrt(per_sm) + 0.5));
     } else {
-        // many rows: whole rounds over the SMs; a cut costs about 3 tiles more (O of 256 rows in 32 bits, twice)
+        // many rows: whole rounds over the SMs, in key tiles of about 2.2 us.  A cut costs an item about 3 tiles more, and
+        // the join reads and the items write O of every row in 32 bits once per split (about 4 TB/s; without that term
+        // 8 prompts behind a prefix of 8192 were cut in two and took 477 us, uncut 439)
+        const double join = (double)a.n_tokens * a.n_heads * (a.pool.head_dim * 8 + 16) / 4e12 / 2.2e-6;
         double best = 1e300;
-        for (int n = 1; n <= 8; ++n) {
+        for (int n = 1; n <= 32; ++n) {
             const long long rounds = (units * n + sms - 1) / sms;
-            const double t = (double)rounds * ((seen + n - 1) / n + 1.5 + (n > 1 ? 3.0 : 0.0));
+            const double t = (double)rounds * ((seen + n - 1) / n + 1.5 + (n > 1 ? 3.0 : 0.0)) + (n > 1 ? n * join : 0.0);
             if (t < best * 0.97) best = t, ct = (seen + n - 1) / n;
         }
     }
