@@ -1645,28 +1645,30 @@ int run_tc(const sd_attn_args& a, int dev, int* err, cudaStream_t st) {
     p.err = err;
     const sd_kv_pool& k = a.pool;
     const bool bf = k.dtype == SD_BF16;
-    const cuuint64_t hd = k.head_dim;
-    {
-        const cuuint64_t dims[3] = {hd, (cuuint64_t)a.n_heads, (cuuint64_t)a.n_tokens};
-        const cuuint64_t strides[2] = {(cuuint64_t)a.q_head * 2, (cuuint64_t)a.q_ld * 2};
-        const cuuint32_t box[3] = {64, (cuuint32_t)p.G, (cuuint32_t)p.TPT};
-        const int rc = encode(&p.tq, bf, 3, a.q, dims, strides, box);
-        if (rc) return rc;
-    }
-    for (int i = 0; i < 2; ++i) {
-        const cuuint32_t rows = std::min(k.page_size, kPaKeys / 2), nh = k.head_dim / 64;
-        const cuuint64_t dims[5] = {64, (cuuint64_t)k.page_size, nh, (cuuint64_t)k.n_kv_heads, (cuuint64_t)k.n_pages};
-        const cuuint64_t strides[4] = {(cuuint64_t)k.pos_stride * 2, 128, (cuuint64_t)k.head_stride * 2, (cuuint64_t)k.page_stride * 2};
-        const cuuint32_t box[5] = {64, rows, i || rows == kPaKeys / 2 ? nh : 1, 1, 1};
-        const int rc = encode(i ? &p.tv : &p.tk, bf, 5, i ? k.v : k.k, dims, strides, box);
-        if (rc) return rc;
-    }
     const int pair = 2 * p.TPT;
     const int own = (a.max_kv + kPaKeys - 1) / kPaKeys + (p.np && a.max_q > pair ? p.np : 0);
     const long long items = (long long)k.n_kv_heads * ((long long)p.cp * p.n_pt + (p.few ? 0LL : (long long)a.n_req + a.n_tokens / pair) *
                                                        std::max(1, (own + p.ct_own - 1) / p.ct_own));
     if (items > INT32_MAX) return fail(SD_ERR_INVALID, "sd_attention_dev: too many work items");
     const int grid = (int)items;
+    if (grid > 0) {  // k_pattn's tensor maps
+        const cuuint64_t hd = k.head_dim;
+        {
+            const cuuint64_t dims[3] = {hd, (cuuint64_t)a.n_heads, (cuuint64_t)a.n_tokens};
+            const cuuint64_t strides[2] = {(cuuint64_t)a.q_head * 2, (cuuint64_t)a.q_ld * 2};
+            const cuuint32_t box[3] = {64, (cuuint32_t)p.G, (cuuint32_t)p.TPT};
+            const int rc = encode(&p.tq, bf, 3, a.q, dims, strides, box);
+            if (rc) return rc;
+        }
+        for (int i = 0; i < 2; ++i) {
+            const cuuint32_t rows = std::min(k.page_size, kPaKeys / 2), nh = k.head_dim / 64;
+            const cuuint64_t dims[5] = {64, (cuuint64_t)k.page_size, nh, (cuuint64_t)k.n_kv_heads, (cuuint64_t)k.n_pages};
+            const cuuint64_t strides[4] = {(cuuint64_t)k.pos_stride * 2, 128, (cuuint64_t)k.head_stride * 2, (cuuint64_t)k.page_stride * 2};
+            const cuuint32_t box[5] = {64, rows, i || rows == kPaKeys / 2 ? nh : 1, 1, 1};
+            const int rc = encode(i ? &p.tv : &p.tk, bf, 5, i ? k.v : k.k, dims, strides, box);
+            if (rc) return rc;
+        }
+    }
     const bool mod = a.softcap > 0.f || a.alibi || !(a.scale > 0.f);
     if (bf) {
         if (k.head_dim == 128) return mod ? launch_tc<__nv_bfloat16, 128, true>(p, grid, dev, st) : launch_tc<__nv_bfloat16, 128, false>(p, grid, dev, st);
