@@ -125,10 +125,14 @@ __global__ void __launch_bounds__(128) k_pattn_general(const sd_attn_args a, int
 // What bounds it.  One causal prompt of 9472 tokens, 32 / 8 heads of 128, no bias: 637 us, 1154 TFLOP/s (0.70 of the
 // measured burst rate of a matrix product, 0.83 of the sustained one, which this length of run is nearer to).  256 rows x
 // 128 keys take the tensor cores 2480 clk with S in halves of 64 keys (N = 64, bound by shared memory; 2050 in one
-// piece, but then a slot's softmax and MMAs alternate: 1.4 x slower overall) and the exponentials 2048 clk; each softmax
-// warp needs about 1900 clk per half, of them 500 to 1000 waiting for its share of the exponentials.  Computing part of
-// these on the FMA pipe (every third to eighth pair) changed nothing or cost up to 5 %; 16 softmax warps of half a row
-// each cost 20 %.  With caps and biases the extra arithmetic per score bounds it.
+// piece) and the exponentials 2048 clk; each softmax warp needs about 1900 clk per half, of them 500 to 1000 waiting for
+// its share of the exponentials.  With caps and biases the extra arithmetic per score bounds it.
+//
+// What the steps measured, each against the kernel as it was then.  S in halves: prompts gained, since a slot's softmax
+// then overlaps its own MMAs (588 -> 550, capped 356 -> 302, biased 476 -> 441 us); single tokens lost (32 over one prefix
+// of 32768 keys 89 -> 97 us, 64 over ragged contexts 410 -> 547 us), and k_pattn_rows serves those now.  Part of the
+// exponentials on the FMA pipe (every third to eighth pair): biased 2 % faster, the others unchanged to 5 % slower, capped
+// 5 to 10 % slower; not kept.  16 softmax warps of half a row each: 570 -> 695 us; not kept.
 // ---------------------------------------------------------------------------------------------
 constexpr int kPaThreads = 384;
 constexpr int kPaKeys = 128;        // keys per tile
