@@ -130,8 +130,8 @@ __global__ void __launch_bounds__(128) k_pattn_general(const sd_attn_args a, int
 //
 // What the steps measured, each against the kernel as it was then.  S in halves: prompts gained, since a slot's softmax
 // then overlaps its own MMAs (588 -> 550, capped 356 -> 302, biased 476 -> 441 us); single tokens lost (32 over one prefix
-// of 32768 keys 89 -> 97 us, 64 over ragged contexts 410 -> 547 us), and k_pattn_rows serves those now.  Part of the
-// exponentials on the FMA pipe (every third to eighth pair): biased 2 % faster, the others unchanged to 5 % slower, capped
+// of 32768 keys 89 -> 97 us, 64 over ragged contexts 410 -> 547 us), and k_pattn_rows serves all but their shared prefix now.
+// With S in halves, part of the exponentials on the FMA pipe (every third to eighth pair): biased 2 % faster, the others unchanged to 5 % slower, capped
 // 5 to 10 % slower; not kept.  16 softmax warps of half a row each: 570 -> 695 us; not kept.
 // ---------------------------------------------------------------------------------------------
 constexpr int kPaThreads = 384;

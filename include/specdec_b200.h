@@ -106,9 +106,10 @@ SD_API int sd_block_sums_dev(const sd_qmat *W, sd_q8_dev x, int32_t *isum, void 
 #define SD_NOALLOC_SCRATCH_BYTES (1u << 20)
 SD_API int sd_matvec_q4_0_q8_0_noalloc_dev(const sd_qmat *W, sd_q8_dev x, float *y, int S, void *stream);
 
-/* Read and clear the error word of `device` that the single-op device entry points above (matvec, block
- * sums, no-alloc matvec) share: 0 if no bounded device wait ran out since the last read, else the positive
- * device error code; negative on a CUDA failure.  Synchronises the device.  No reference counterpart (the
+/* Read and clear the error word of `device` that the single-op device entry points (matvec, block sums, no-alloc
+ * matvec, and the paged cache's below) share: 0 if no bounded device wait ran out and no page, slot or length was
+ * left out as out of range (code 3) since the last read, else the positive device error code; negative on a CUDA
+ * failure.  Synchronises the device.  No reference counterpart (the
  * reference's CPU calls cannot time out). */
 SD_API int sd_device_error(int device);
 
