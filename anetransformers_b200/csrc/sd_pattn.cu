@@ -1704,6 +1704,7 @@ int check_attention(const sd_attn_args* a) {
         return fail(SD_ERR_INVALID, "%s: scale %g, softcap %g", what, a->scale, a->softcap);
     if (a->q_head < a->pool.head_dim || a->out_head < a->pool.head_dim || a->q_ld < 0 || a->out_ld < 0)
         return fail(SD_ERR_INVALID, "%s: strides", what);
+    if (a->n_tokens > 1 && a->out_ld < a->pool.head_dim) return fail(SD_ERR_INVALID, "%s: the tokens of out overlap", what);
     return SD_OK;
 }
 

@@ -206,7 +206,7 @@ typedef struct {
     sd_kv_pool pool;
     const void *q;
     void *out;
-    int64_t q_ld, q_head, out_ld, out_head; /* elements between tokens, between heads */
+    int64_t q_ld, q_head, out_ld, out_head; /* elements between tokens, between heads; rows of out do not overlap */
     const int32_t *table, *kv_len, *q_start, *q_len;
     const int32_t *prefix_table; /* [ceil(prefix_len / page_size)], NULL if prefix_len is 0 */
     const float *alibi;          /* [n_heads] or NULL */

@@ -108,3 +108,8 @@ def test_shared_batch_refusals():
                  (P, P, 4, 2, 64, 0), (P, P, 4, 2, 64, 9), (P, P, 1 << 30, 2, 64, 5)]:
         refused(L.sd_batch_create_shared(*args, C.byref(out)))
     refused(L.sd_batch_create_shared(P, P, 4, 2, 64, 5, None))
+
+
+@pytest.mark.parametrize("out_ld", [0, 64, 127])
+def test_out_rows_that_overlap(out_ld):
+    refused(_lib.lib().sd_attention_dev(C.byref(attn(out_ld=out_ld, n_tokens=2)), None), "overlap")
