@@ -10,6 +10,7 @@
 
 #include <algorithm>
 #include <atomic>
+#include <cfloat>
 #include <cmath>
 #include <type_traits>
 
@@ -1263,6 +1264,7 @@ __global__ void __launch_bounds__(kRwThreads) k_pattn_rows(const __grid_constant
     float slope[NT][2];
     const float kLog2e = 1.4426950408889634f, sc2 = a.scale * kLog2e;
     const float cap2 = a.softcap * kLog2e, x1 = a.softcap > 0.f ? a.scale / a.softcap : 0.f;
+    const CapPoly kcap = cap_poly(cap2);
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
@@ -1310,18 +1312,37 @@ __global__ void __launch_bounds__(kRwThreads) k_pattn_rows(const __grid_constant
         uint32_t pf[NT][2];
         float fac[NT][2];
         bool rise = false;
+        if (a.softcap > 0.f) {
+            // as in k_pattn, the same choice for each score whatever its neighbours are: the quotient's error is a part of
+            // the cap, so small scores take the polynomial, whose error is a part of the score
+            float2 x[NT][2];
+            bool big = false;
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+                for (int e = 0; e < 2; ++e) {
+                    x[nt][e] = __fmul2_rn(make_float2(sc[nt][2 * e], sc[nt][2 * e + 1]), make_float2(x1, x1));
+                    const float2 z = cap_small(x[nt][e], kcap);
+                    sc[nt][2 * e] = z.x;
+                    sc[nt][2 * e + 1] = z.y;
+                    big |= !(fabsf(x[nt][e].x) <= 0.5f) || !(fabsf(x[nt][e].y) <= 0.5f);
+                }
+            if (__any_sync(0xffffffffu, big)) {
+#pragma unroll
+                for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) {
+                        const float y = e & 1 ? x[nt][e >> 1].y : x[nt][e >> 1].x;
+                        if (!(fabsf(y) <= 0.5f)) sc[nt][e] = fmaf(rcp(1.f + ex2(y * (2.f * kLog2e))), -2.f * cap2, cap2);
+                    }
+            }
+        }
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt) {
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
                 const int k = kg + (e >> 1) * 8, stop = end[nt][e & 1];
-                float z;
-                if (a.softcap > 0.f) {
-                    const float x = sc[nt][e] * x1;
-                    z = fmaf(rcp(1.f + ex2(x * (2.f * kLog2e))), -2.f * cap2, cap2);
-                } else {
-                    z = sc[nt][e] * sc2;
-                }
+                float z = a.softcap > 0.f ? sc[nt][e] : sc[nt][e] * sc2;
                 if (a.alibi) z = fmaf(slope[nt][e & 1], (float)(k - (stop - 1)), z);
                 if (!there || k >= stop || (W > 0 && k < stop - W)) z = -INFINITY;
                 sc[nt][e] = z;
@@ -1502,9 +1523,11 @@ EncodeTiled encode_tiled() {
     return fn;
 }
 
-// What TMA and 16-byte accesses need; other calls take the general kernel.
+// What TMA and 16-byte accesses need, and a scale / cap that 32 bits hold in full (the scores are multiplied by it at once);
+// other calls take the general kernel.
 bool tc_able(const sd_attn_args& a) {
     const sd_kv_pool& k = a.pool;
+    if (a.softcap > 0.f && a.scale != 0.f && !(std::fabs(a.scale / a.softcap) >= FLT_MIN)) return false;
     auto al = [](const void* q) { return (reinterpret_cast<uintptr_t>(q) & 15) == 0; };
     auto st = [](int64_t s) { return s > 0 && s % 8 == 0 && s < (1ll << 38); };
     return (k.head_dim == 64 || k.head_dim == 128) && al(k.k) && al(k.v) && al(a.q) && al(a.out) && st(k.page_stride) &&

@@ -201,7 +201,8 @@ SD_API int sd_kv_append_dev(const sd_kv_pool *pool, const void *k, const void *v
  * q_start ascends, the ranges do not overlap and end within n_tokens.  max_q and max_kv bound q_len and kv_len on the
  * host (they size the launch; a tight max_kv gives the better split); a longer request is cut there (recorded).
  * head_dim a multiple of 8 up to 256 (64 and 128 with 16-byte aligned rows run on the tensor cores), n_heads a multiple of
- * n_kv_heads (at most 128 per kv head), q and out of the pool's type and not overlapping; softcap 0 or 1e-6..1e30. */
+ * n_kv_heads (at most 128 per kv head), q and out of the pool's type and not overlapping; softcap 0 or 1e-6..1e30 (capped
+ * scores are right to 2^-20 of their value; where scale / softcap is below 2^-126 the plain kernel takes the call). */
 typedef struct {
     sd_kv_pool pool;
     const void *q;
