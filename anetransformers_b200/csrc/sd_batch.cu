@@ -563,13 +563,14 @@ __global__ void __launch_bounds__(kBCombWarps * 32) k_bq8(const __half* x, WImg 
     store_q8_head(img, m, h, lane, o);
 }
 
-// Lengths of a forward for the page plan: stream b has pos + nv positions behind the prefix, nv of them new (a finished
-// stream keeps its positions); row n is the prefix itself.
-__global__ void k_bpage_lens(const DevCtrl* ctrl, int n, int T, int prefix, int* kv_len, int* q_len) {
+// Lengths of a forward for the page plan: stream b has pos + nv positions behind the prefix, nv of them new; row n is the
+// prefix itself.  A stream that has finished keeps every page it holds (its control block still has the position of its last
+// forward's first token, so that position would give back the pages of that forward's tokens).
+__global__ void k_bpage_lens(const DevCtrl* ctrl, int n, int T, int prefix, int max_seq, int page, const int* held, int* kv_len, int* q_len) {
     const int b = blockIdx.x * blockDim.x + threadIdx.x;
     if (b > n) return;
     const int nv = b == n || ctrl[b].done ? 0 : min(ctrl[b].n_valid, T);
-    kv_len[b] = b == n ? prefix : ctrl[b].pos + nv;
+    kv_len[b] = b == n ? prefix : ctrl[b].done ? min(held[b] * page, max_seq) : ctrl[b].pos + nv;
     q_len[b] = nv;
 }
 
@@ -878,7 +879,8 @@ int enqueue_bforward(sd_batch* b, int T, bool logits) {
     CK(cudaGetLastError(), "embed");
     if (b->paged) {
         if (!b->filling) {
-            k_bpage_lens<<<b->B / 128 + 1, 128, 0, b->st>>>(b->ctrl, b->B, T, b->prefix, b->kv_len, b->q_len);
+            k_bpage_lens<<<b->B / 128 + 1, 128, 0, b->st>>>(b->ctrl, b->B, T, b->prefix, b->max_seq, kPage, b->pages.held, b->kv_len,
+                                                               b->q_len);
             CK(cudaGetLastError(), "lengths");
         }
         // the prefix's slices are one request's tokens in a row, a stream's are T apart

@@ -484,7 +484,8 @@ SD_API int sd_batch_forward(sd_batch *b, const int32_t *tokens, int T, const int
  * computed here once and kept once, and every forward's attention reads it once for the rows of all streams.  K/V lives
  * in pages (sd_pages, sd_attention_dev) instead of one ring per stream.  Every sd_batch_* call works on it, counting a
  * stream's positions from the end of the prefix (position 0 is the first token behind it); max_seq is their number.
- * A forward gives back the pages of positions behind its last token; a stream's n-gram history and repetition window
+ * A forward gives back the pages of positions behind its last token (a stream that has finished while others decode keeps
+ * its own); a stream's n-gram history and repetition window
  * do not reach into the prefix.  Logits agree with those of a plain batch over prefix + tokens within the batched path's
  * tolerance (5e-3 relative): both attend with single fp16 Q and P. */
 SD_API int sd_batch_create_shared(sd_ctx *ctx, const int32_t *prefix, int n_prefix, int n_streams, int max_seq,
