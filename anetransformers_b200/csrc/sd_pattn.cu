@@ -213,9 +213,24 @@ __device__ __forceinline__ int pa_request(const sd_attn_args& a, int tok) {
     return lo;
 }
 
+// First prefix position that a row of a prefix item sees through the window: from the least position of its rows that have
+// one, but for inline requests', whose prefix is in their own items.  A whole warp does this, a request per lane.
+__device__ __forceinline__ int pa_prefix_first(const PaArgs& p, const PaItem& it, int lane) {
+    const sd_attn_args& a = p.a;
+    const int P = a.prefix_len, last = pa_request(a, it.tok0 + it.ntok - 1);
+    int low = INT32_MAX;
+    for (int b = pa_request(a, it.tok0) + lane; b <= last; b += 32) {
+        const int rows = pa_rows(a, b), base = pa_kv(a, b) - pa_q(a, b);
+        const int t0 = max(0, it.tok0 - a.q_start[b]), t1 = min(rows, it.tok0 + it.ntok - a.q_start[b]);
+        if (t0 < t1 && base + t1 > 0 && !pa_inline(p, rows)) low = min(low, max(0, base + t0));
+    }
+    low = __reduce_min_sync(0xffffffffu, low);
+    return low == INT32_MAX ? P : min(P, max(0, P + low + 1 - a.window));
+}
+
 // Item number i of the launch; false if it holds nothing (prefix rows of an inline request).  The TMA warp does this, ahead
 // of the others; they read the result.
-__device__ __forceinline__ bool pa_item(const PaArgs& p, const int* ustart, int i, PaItem& it) {
+__device__ __forceinline__ bool pa_item(const PaArgs& p, const int* ustart, int i, int lane, PaItem& it) {
     const sd_attn_args& a = p.a;
     const int n_kv = a.pool.n_kv_heads, P = a.prefix_len, W = a.window;
     const int n_pre = p.cp * p.n_pt * n_kv;
@@ -232,7 +247,7 @@ __device__ __forceinline__ bool pa_item(const PaArgs& p, const int* ustart, int 
         it.pair = it.ntok > p.TPT;
         it.direct = false;
         it.npt = p.np;
-        it.klo_p = W > 0 ? max(0, P + 1 - W) : 0;
+        it.klo_p = W > 0 ? pa_prefix_first(p, it, lane) : 0;
         it.klo_o = it.khi_o = 0;
         it.v0 = max(c * p.ct_pre, it.klo_p / kPaKeys);
         it.n = max(0, min(p.np, (c + 1) * p.ct_pre) - it.v0);
@@ -264,7 +279,8 @@ __device__ __forceinline__ bool pa_item(const PaArgs& p, const int* ustart, int 
     it.pair = it.ntok > p.TPT;
     it.direct = chunks == 1 && (P == 0 || inl);
     it.npt = inl ? p.np : 0;
-    const int first = it.base + tile * 2 * p.TPT, last = first + it.ntok - 1;
+    const int last = it.base + tile * 2 * p.TPT + it.ntok - 1;
+    const int first = max(0, it.base + tile * 2 * p.TPT);  // of the rows that have a position
     it.khi_o = max(0, last + 1);
     it.klo_o = W > 0 ? max(0, first + 1 - W) : 0;
     it.klo_p = W > 0 ? min(P, max(0, P + first + 1 - W)) : 0;
@@ -603,7 +619,7 @@ __global__ void __launch_bounds__(kPaThreads, 1) k_pattn(const __grid_constant__
             if (next >= 0) {
                 if (lane == 0) pa_claim(ctl);
                 open = true;
-                if (!pa_item(p, ustart, next, it)) {
+                if (!pa_item(p, ustart, next, lane, it)) {
                     claimed();
                     continue;
                 }

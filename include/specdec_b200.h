@@ -195,8 +195,8 @@ SD_API int sd_kv_append_dev(const sd_kv_pool *pool, const void *k, const void *v
  * then - alibi[head] * distance if alibi is not NULL; softmax and the weighted sum of V are accumulated in fp32, the
  * softmax weights enter the product with V in the pool's type.
  * A row with i < 0, or with nothing to see, is 0.  Tokens of no request are left as they were.  Positions whose page
- * id is outside the pool are not seen (recorded, unless all that every row of the call would see of the page is
- * outside the window).  K and V of positions that no row sees may hold anything; those that some row of the request
+ * id is outside the pool are not seen (recorded, unless the page lies outside the windows of all rows of the call).  K and
+ * V of positions that no row sees may hold anything; those that some row of the request (of the prefix: of the call)
  * sees must be finite.
  * q_start ascends, the ranges do not overlap and end within n_tokens.  max_q and max_kv bound q_len and kv_len on the
  * host (they size the launch; a tight max_kv gives the better split); a longer request is cut there (recorded).
