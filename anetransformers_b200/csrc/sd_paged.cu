@@ -101,20 +101,21 @@ __global__ void __launch_bounds__(kPlanThreads) k_pages_plan(const PlanArgs a) {
     const cg::cluster_group cluster = cg::this_cluster();
     const int gtid = (int)cluster.block_rank() * kPlanThreads + tid, gn = (int)cluster.num_blocks() * kPlanThreads;
     const int cap = a.table_ld * a.page_size;
-    const int count0 = *a.n_free;
+    const int free0 = *a.n_free, count0 = min(max(free0, 0), a.n_pages), room = a.n_pages - count0;
 
     // sums: each thread takes `per` consecutive requests
     const int per = (n + kPlanThreads - 1) / kPlanThreads;
     const int b0 = min(n, tid * per), b1 = min(n, b0 + per);
     int s[3] = {0, 0, 0};
-    bool bad = false;
+    bool bad = free0 != count0;
     for (int b = b0; b < b1; ++b) {
         int kv = a.kv_len[b], q = a.q_len[b];
         if (kv < 0 || kv > cap) bad = true, kv = min(max(kv, 0), cap);
         const int q_max = a.q_stride > 0 ? a.q_stride : a.n_tokens;
         if (q < 0 || q > q_max) bad = true, q = min(max(q, 0), q_max);
         if (a.q_stride > 0 && q > 0 && b * a.q_stride + q > a.n_tokens) bad = true;
-        const int need = (kv + a.page_size - 1) / a.page_size, had = min(max(a.held[b], 0), a.table_ld);
+        const int need = (kv + a.page_size - 1) / a.page_size, held = a.held[b], had = min(max(held, 0), a.table_ld);
+        if (held != had) bad = true;
         const int v[3] = {max(had - need, 0), max(need - had, 0), q};
         back[b] = v[0], want[b] = v[1], toks[b] = v[2];
         base[b] = min(had, need);
@@ -155,25 +156,26 @@ __global__ void __launch_bounds__(kPlanThreads) k_pages_plan(const PlanArgs a) {
     }
     __syncthreads();
     const int n_back = tot[0], n_want = tot[1], n_tok = tot[2];
-    const int count = min(count0 + n_back, a.n_pages), left = max(count - n_want, 0);
+    const int count = count0 + min(n_back, room), left = max(count - n_want, 0);
+    if (n_back > room) bad = true;  // the stack would hold more pages than there are
     if (n_back | n_want) {
         cluster.sync();  // every CTA has read the old state
-        for (int k0 = gtid; k0 < n_back; k0 += 4 * gn) {
+        for (unsigned k0 = gtid; k0 < (unsigned)n_back; k0 += 4 * gn) {
             size_t i[4];
             int page[4];
 #pragma unroll
             for (int u = 0; u < 4; ++u) {
-                const int k = k0 + u * gn;
-                if (k >= n_back) continue;
-                const int b = owner(back, n, k);
-                i[u] = (size_t)b * a.table_ld + base[b] + (k - back[b]);
+                const unsigned k = k0 + u * gn;
+                if (k >= (unsigned)n_back) continue;
+                const int b = owner(back, n, (int)k);
+                i[u] = (size_t)b * a.table_ld + base[b] + ((int)k - back[b]);
                 page[u] = a.table[i[u]];
             }
 #pragma unroll
             for (int u = 0; u < 4; ++u) {
-                const int k = k0 + u * gn;
-                if (k >= n_back) continue;
-                if (count0 + k < a.n_pages) a.free_pages[count0 + k] = page[u];
+                const unsigned k = k0 + u * gn;
+                if (k >= (unsigned)n_back) continue;
+                if (k < (unsigned)room) a.free_pages[count0 + k] = page[u];
                 a.table[i[u]] = -1;
             }
         }
