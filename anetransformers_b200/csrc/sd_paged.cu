@@ -229,7 +229,8 @@ __global__ void __launch_bounds__(kPlanThreads) k_pages_plan(const PlanArgs a) {
             if (p >= 0 && p < cap) {
                 pos = a.pos0 + p;
                 const int page = a.table[(size_t)b * a.table_ld + p / a.page_size];
-                if (page >= 0) slot = page * a.page_size + p % a.page_size;
+                if (page >= 0 && page < a.n_pages) slot = page * a.page_size + p % a.page_size;
+                else if (page != -1) bad = true;
             }
         }
         a.slots[k] = slot;

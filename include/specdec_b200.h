@@ -164,7 +164,8 @@ SD_API int sd_pages_reset_dev(const sd_pages *p, void *stream);
  * Tokens: the new positions of request b are tokens q_start[b] .. q_start[b] + q_len[b) of the step, packed one
  * request after another (q_stride 0) or at b * q_stride (q_len <= q_stride).  slots [n_tokens]: token's slot in the
  * pool, page * page_size + offset; positions [n_tokens] (or NULL): pos0 + its position.  Tokens of no request get -1
- * in both; a position that has no page gets slot -1, one before 0 (q_len > kv_len) -1 in both.
+ * in both; a position that has no page gets slot -1 (as does one whose page id is none of the pool's: recorded), one
+ * before 0 (q_len > kv_len) -1 in both.
  * q_len = 0 keeps a request's pages, kv_len = 0 releases them.  A length past table_ld * page_size is cut there, a
  * q_len outside 0 .. q_stride to that range, tokens past n_tokens are dropped; a *n_free outside 0 .. n_pages or a held[b]
  * outside 0 .. table_ld counts as the nearest of these, and pages given back that the stack has no room for are dropped.
