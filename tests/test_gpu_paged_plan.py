@@ -91,7 +91,7 @@ def test_page_ids_out_of_the_pool(pg):
     """A free stack that names pages that do not exist: no slot is made of them."""
     pool = pg.PagePool(2, 8, 16, 64)
     pool.free[6:] = i32([8, 1 << 28])  # the next two pages taken: 2^28 (whose slots would wrap to 0 and on), then 8
-    got = pool.plan(i32([3, 18]), i32([3, 18]), 21)  # request 1's second page is page 5
+    got = pool.plan(i32([3, 18]), i32([3, 18]), 21)  # request 1 gets page 8, which is none, then free[5] = 2
     assert error_word() == 3
-    assert got.slots.tolist() == [-1] * 19 + [5 * 16, 5 * 16 + 1]
+    assert got.slots.tolist() == [-1] * 19 + [2 * 16, 2 * 16 + 1]
     assert got.positions.tolist() == list(range(3)) + list(range(18))
