@@ -80,6 +80,9 @@ struct PlanArgs {
     int* err;
 };
 
+// Sum of two that are not negative, at most INT32_MAX (so that sums of lengths out of range still ascend).
+__device__ __forceinline__ int add_sat(int x, int y) { return (int)min((unsigned)x + (unsigned)y, (unsigned)INT32_MAX); }
+
 // Last b in [0, n) with start[b] <= k (start ascends, start[0] = 0).
 __device__ __forceinline__ int owner(const int* start, int n, int k) {
     int lo = 0, hi = n;
@@ -120,7 +123,7 @@ __global__ void __launch_bounds__(kPlanThreads) k_pages_plan(const PlanArgs a) {
         back[b] = v[0], want[b] = v[1], toks[b] = v[2];
         base[b] = min(had, need);
 #pragma unroll
-        for (int i = 0; i < 3; ++i) s[i] += v[i];
+        for (int i = 0; i < 3; ++i) s[i] = add_sat(s[i], v[i]);
     }
     int incl[3];
 #pragma unroll
@@ -129,7 +132,7 @@ __global__ void __launch_bounds__(kPlanThreads) k_pages_plan(const PlanArgs a) {
 #pragma unroll
         for (int o = 1; o < 32; o <<= 1) {
             const int u = __shfl_up_sync(0xffffffffu, incl[i], o);
-            if (lane >= o) incl[i] += u;
+            if (lane >= o) incl[i] = add_sat(incl[i], u);
         }
         if (lane == 31) wsum[i][warp] = incl[i];
     }
@@ -141,16 +144,17 @@ __global__ void __launch_bounds__(kPlanThreads) k_pages_plan(const PlanArgs a) {
 #pragma unroll
         for (int w = 0; w < kPlanThreads / 32; ++w) {
             const int u = wsum[i][w];
-            before += w < warp ? u : 0;
-            all += u;
+            before = w < warp ? add_sat(before, u) : before;
+            all = add_sat(all, u);
         }
         tot[i] = all;
-        int run = before + incl[i] - s[i];
+        const int up = __shfl_up_sync(0xffffffffu, incl[i], 1);  // of the lanes in front
+        int run = lane ? add_sat(before, up) : before;
         int* arr = i == 0 ? back : i == 1 ? want : toks;
         for (int b = b0; b < b1; ++b) {
             const int v = arr[b];
             arr[b] = run;
-            run += v;
+            run = add_sat(run, v);
         }
         if (tid == 0) arr[n] = all;
     }
@@ -211,7 +215,8 @@ __global__ void __launch_bounds__(kPlanThreads) k_pages_plan(const PlanArgs a) {
         if (a.q_stride == 0 && n_tok > a.n_tokens) bad = true;
     }
     for (int b = gtid; b < n; b += gn) a.q_start[b] = a.q_stride > 0 ? b * a.q_stride : toks[b];
-    for (int k = gtid; k < a.n_tokens; k += gn) {
+    for (unsigned u = gtid; u < (unsigned)a.n_tokens; u += gn) {
+        const int k = (int)u;
         int b, t;
         bool live;
         if (a.q_stride > 0) {
@@ -224,8 +229,10 @@ __global__ void __launch_bounds__(kPlanThreads) k_pages_plan(const PlanArgs a) {
             live = true;
         }
         int slot = -1, pos = -1;
-        if (live && t >= 0 && t < toks[b + 1] - toks[b]) {
-            const int p = min(a.kv_len[b], cap) - (toks[b + 1] - toks[b]) + t;
+        int q = live ? toks[b + 1] - toks[b] : 0;
+        if (live && toks[b + 1] == INT32_MAX) q = min(max(a.q_len[b], 0), a.q_stride > 0 ? a.q_stride : a.n_tokens);
+        if (t >= 0 && t < q) {
+            const int p = min(a.kv_len[b], cap) - q + t;
             if (p >= 0 && p < cap) {
                 pos = a.pos0 + p;
                 const int page = a.table[(size_t)b * a.table_ld + p / a.page_size];

@@ -95,3 +95,14 @@ def test_page_ids_out_of_the_pool(pg):
     assert error_word() == 3
     assert got.slots.tolist() == [-1] * 19 + [2 * 16, 2 * 16 + 1]
     assert got.positions.tolist() == list(range(3)) + list(range(18))
+
+
+def test_more_new_tokens_than_32_bits_count(pg):
+    """Lengths that add up past 2^31: the tokens that have room are those of the first requests, the others are dropped."""
+    n, room = 4096, 1 << 20
+    pool = pg.PagePool(n, 64, 16, 64)
+    got = pool.plan(i32([5] + [0] * (n - 1)), i32([5] + [room] * (n - 1)), room)
+    assert error_word() == 3
+    assert got.positions[:5].tolist() == list(range(5)) and got.slots[:5].tolist() == list(range(5))
+    assert bool((got.slots[5:] == -1).all())
+    assert got.q_start[:3].tolist() == [0, 5, 5 + room]
