@@ -4,6 +4,7 @@
 #include <cuda_bf16.h>
 
 #include <algorithm>
+#include <atomic>
 
 #include "sd_common.cuh"
 #include "sd_host.h"
@@ -70,6 +71,8 @@ namespace {
 // by 64 others, 36 thousand tokens: 15 us (59 us by one CTA).
 // ---------------------------------------------------------------------------------------------
 constexpr int kPlanThreads = 512;
+
+constexpr size_t plan_smem(int n_req) { return ((size_t)4 * n_req + 3) * sizeof(int); }
 
 struct PlanArgs {
     int32_t *table, *held, *free_pages, *n_free;
@@ -353,11 +356,19 @@ int launch_pages_plan(const sd_pages* p, const int32_t* kv_len, const int32_t* q
                       int32_t* q_start, int32_t* slots, int32_t* positions, int32_t* missing, int* err, cudaStream_t st) {
     PlanArgs a{p->table, p->held, p->free_pages, p->n_free, p->n_req, p->table_ld, p->n_pages, p->page_size,
                kv_len, q_len, q_stride, pos0, n_tokens, q_start, slots, positions, missing, err};
-    const size_t smem = ((size_t)4 * p->n_req + 3) * sizeof(int);
+    const size_t smem = plan_smem(p->n_req);
     cudaError_t e = cudaSuccess;
-    if (smem > 48 * 1024 - 1024)
-        e = cudaFuncSetAttribute(k_pages_plan, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
-    if (e != cudaSuccess) return cuda_fail(e, "pages plan");
+    if (smem > 48 * 1024 - 1024) {
+        // once per device, to the largest batch's: another thread's smaller batch must not lower it in front of a launch
+        static std::atomic<bool> ready[64];
+        int dev = 0;
+        if ((e = cudaGetDevice(&dev)) != cudaSuccess) return cuda_fail(e, "pages plan");
+        if (dev < 0 || dev >= 64 || !ready[dev].load(std::memory_order_acquire)) {
+            e = cudaFuncSetAttribute(k_pages_plan, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)plan_smem(SD_PAGES_MAX_REQ));
+            if (e != cudaSuccess) return cuda_fail(e, "pages plan");
+            if (dev >= 0 && dev < 64) ready[dev].store(true, std::memory_order_release);
+        }
+    }
     // a thread's share of a step is a token or a few pages of a request (the host does not know how many move)
     const long long items = std::max<long long>(n_tokens, 16LL * p->n_req);
     int ctas = 1;

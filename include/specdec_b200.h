@@ -167,9 +167,9 @@ SD_API int sd_pages_reset_dev(const sd_pages *p, void *stream);
  * in both; a position that has no page gets slot -1 (as does one whose page id is none of the pool's: recorded), one
  * before 0 (q_len > kv_len) -1 in both.
  * q_len = 0 keeps a request's pages, kv_len = 0 releases them.  A length past table_ld * page_size is cut there, a
- * q_len outside 0 .. q_stride to that range, tokens past n_tokens are dropped (q_start counts to 2^31 - 1); a *n_free outside 0 .. n_pages or a held[b]
- * outside 0 .. table_ld counts as the nearest of these, and pages given back that the stack has no room for are dropped.
- * Each records DEV error 3. */
+ * q_len outside 0 .. q_stride to that range, tokens past n_tokens are dropped (q_start counts to 2^31 - 1); a *n_free
+ * outside 0 .. n_pages or a held[b] outside 0 .. table_ld counts as the nearest of these, and pages given back that the
+ * stack has no room for are dropped.  Each records DEV error 3. */
 SD_API int sd_pages_plan_dev(const sd_pages *p, const int32_t *kv_len, const int32_t *q_len, int q_stride, int pos0,
                              int n_tokens, int32_t *q_start, int32_t *slots, int32_t *positions, int32_t *missing,
                              void *stream);

@@ -1,5 +1,6 @@
 """The page plan's checks of what only the device knows: entries out of range are left out and recorded (code 3)."""
 import ctypes as C
+import threading
 
 import pytest
 
@@ -106,3 +107,27 @@ def test_more_new_tokens_than_32_bits_count(pg):
     assert got.positions[:5].tolist() == list(range(5)) and got.slots[:5].tolist() == list(range(5))
     assert bool((got.slots[5:] == -1).all())
     assert got.q_start[:3].tolist() == [0, 5, 5 + room]
+
+
+def test_large_batches_from_two_threads(pg):
+    """Two host threads that plan large batches of different sizes, each on a pool and a stream of its own."""
+    import torch
+    from anetransformers_b200 import _lib
+    plan, failed = _lib.lib().sd_pages_plan_dev, []
+
+    def loop(n):
+        with torch.cuda.stream(torch.cuda.Stream()):
+            pool = pg.PagePool(n, n, 16, 16)
+            kv, q, q_start = i32([1] * n), i32([0] * n), i32([0] * n)
+            c = _lib.Pages(pool.table.data_ptr(), pool.held.data_ptr(), pool.free.data_ptr(), pool.n_free.data_ptr(), n, 1, n, 16)
+            args = (C.byref(c), kv.data_ptr(), q.data_ptr(), 0, 0, 0, q_start.data_ptr(), None, None, None,
+                    torch.cuda.current_stream().cuda_stream)
+            failed.extend(rc for rc in (plan(*args) for _ in range(20000)) if rc)
+            torch.cuda.current_stream().synchronize()
+            failed.extend(x for x in pool.held.tolist() if x != 1)
+    threads = [threading.Thread(target=loop, args=(n,)) for n in (4096, 3100)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not failed
