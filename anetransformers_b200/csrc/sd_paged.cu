@@ -420,7 +420,7 @@ int sd_kv_append_dev(const sd_kv_pool* pool, const void* k, const void* v, int s
     clear_error();
     int rc = check_kv_pool(pool, "sd_kv_append_dev"), dev;
     if (rc) return rc;
-    if (!k || !v || !slots || n_tokens < 0) return fail(SD_ERR_INVALID, "sd_kv_append_dev: bad arguments");
+    if (n_tokens < 0 || (n_tokens > 0 && (!k || !v || !slots))) return fail(SD_ERR_INVALID, "sd_kv_append_dev: bad arguments");
     if (src_dtype != SD_F32 && src_dtype != pool->dtype)
         return fail(SD_ERR_INVALID, "sd_kv_append_dev: source type %d for a pool of type %d", src_dtype, pool->dtype);
     if (n_tokens == 0) return SD_OK;

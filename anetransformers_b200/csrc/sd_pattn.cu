@@ -1726,7 +1726,7 @@ int check_attention(const sd_attn_args* a) {
     if (!a) return fail(SD_ERR_INVALID, "%s: null arguments", what);
     int rc = check_kv_pool(&a->pool, what);
     if (rc) return rc;
-    if (!a->q || !a->out || !a->table || !a->kv_len || !a->q_start || !a->q_len)
+    if ((a->n_tokens != 0 && (!a->q || !a->out)) || !a->table || !a->kv_len || !a->q_start || !a->q_len)
         return fail(SD_ERR_INVALID, "%s: null argument", what);
     if (a->n_req < 1 || a->n_req > SD_PAGES_MAX_REQ)
         return fail(SD_ERR_INVALID, "%s: n_req %d outside 1..%d", what, a->n_req, SD_PAGES_MAX_REQ);

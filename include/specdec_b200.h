@@ -186,7 +186,7 @@ typedef struct {
 /* Write token i's K and V rows ([n_kv_heads][head_dim], heads head_dim apart, tokens k_ld / v_ld elements apart) into
  * slot slots[i], rounded to the pool's type.  src_dtype: SD_F32 or the pool's.  Slot -1 is skipped, any other slot
  * outside the pool is skipped and recorded.  Slots of one call must differ: of tokens with the same slot an
- * unspecified mix stays. */
+ * unspecified mix stays.  Without tokens k, v and slots may be NULL. */
 SD_API int sd_kv_append_dev(const sd_kv_pool *pool, const void *k, const void *v, int src_dtype, int64_t k_ld,
                             int64_t v_ld, const int32_t *slots, int n_tokens, void *stream);
 
@@ -197,6 +197,7 @@ SD_API int sd_kv_append_dev(const sd_kv_pool *pool, const void *k, const void *v
  * is below `window` (0: no limit).  Its scores are scale * q.k, then softcap * tanh(score / softcap) if softcap > 0,
  * then - alibi[head] * distance if alibi is not NULL; softmax and the weighted sum of V are accumulated in fp32, the
  * softmax weights enter the product with V in the pool's type.
+ * Without tokens (n_tokens 0) there is nothing to do, and q and out may be NULL.
  * A row with i < 0, or with nothing to see, is 0.  Tokens of no request are left as they were.  Positions whose page
  * id is outside the pool are not seen (recorded, unless the page lies outside the windows of all rows of the call).  K and
  * V of positions that no row sees may hold anything; those that some row of the request (of the prefix: of the call)
