@@ -28,6 +28,13 @@ def _refuse(msg: str):
     raise _lib.SpecDecError(_ERR_INVALID, msg)
 
 
+def _sizes(**kw):
+    """Sizes as the C calls take them: ctypes would cut a wider integer to its low 32 bits."""
+    for name, v in kw.items():
+        if not 0 <= v <= 0x7FFFFFFF:
+            _refuse(f"{name} {v} outside 0..2^31-1")
+
+
 def _i32(name, t, numel=None):
     if t.dtype is not torch.int32:
         _refuse(f"{name} must be int32, not {t.dtype}")
@@ -70,7 +77,7 @@ class PagePool:
     the table is the prefix_table of attention_dev."""
 
     def __init__(self, n_req: int, n_pages: int, page_size: int, max_len: int, device="cuda"):
-        if n_req < 1 or n_pages < 1 or max_len < 1 or page_size < 1:
+        if not all(1 <= x <= 0x7FFFFFFF for x in (n_req, n_pages, page_size, max_len)):
             _refuse(f"PagePool({n_req}, {n_pages}, {page_size}, {max_len})")
         self.page_size = page_size
         self.table = torch.empty(n_req, -(-max_len // page_size), dtype=torch.int32, device=device)
@@ -89,6 +96,7 @@ class PagePool:
     def plan(self, kv_len, q_len, n_tokens: int, q_stride: int = 0, pos0: int = 0, out: Optional[Plan] = None) -> Plan:
         """Pages and slots of one step (sd_pages_plan_dev): kv_len [n_req] positions after it, q_len [n_req] new ones."""
         n, dev = self._c.n_req, self.table.device
+        _sizes(n_tokens=n_tokens, q_stride=q_stride, pos0=pos0)
         if out is None:
             buf = torch.empty(n + 2 * n_tokens + 1, dtype=torch.int32, device=dev)
             out = Plan(*buf.split_with_sizes((n, n_tokens, n_tokens, 1)))
@@ -131,6 +139,7 @@ def attention_dev(q, k_pages, v_pages, table, kv_len, q_start, q_len, *, max_q: 
     prefix_table: pages of the prefix_len positions that every request shares; alibi [n_heads] fp32 slopes.
     Tokens of no request are left as out has them."""
     pool = _kv_pool(k_pages, v_pages)
+    _sizes(max_q=max_q, max_kv=max_kv, prefix_len=prefix_len, window=window)
     if q.dim() != 3 or q.shape[2] != pool.head_dim or q.dtype is not k_pages.dtype or q.stride(2) != 1:
         _refuse(f"q {tuple(q.shape)} {q.dtype} over pages of [{pool.n_kv_heads}, {pool.head_dim}] {k_pages.dtype}")
     if out is None:
