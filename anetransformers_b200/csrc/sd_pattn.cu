@@ -214,18 +214,24 @@ __device__ __forceinline__ int pa_request(const sd_attn_args& a, int tok) {
 }
 
 // First prefix position that a row of a prefix item sees through the window: from the least position of its rows that have
-// one, but for inline requests', whose prefix is in their own items.  A whole warp does this, a request per lane.
-__device__ __forceinline__ int pa_prefix_first(const PaArgs& p, const PaItem& it, int lane) {
+// one, but for inline requests', whose prefix is in their own items.  A whole warp does this, a request per lane.  (A call
+// of its own: inlined, it cost calls without a window 2 to 3 % by the code around it.)
+__device__ __noinline__ int pa_prefix_first(const PaArgs& p, int tok0, int ntok, int lane) {
     const sd_attn_args& a = p.a;
-    const int P = a.prefix_len, last = pa_request(a, it.tok0 + it.ntok - 1);
-    int low = INT32_MAX;
-    for (int b = pa_request(a, it.tok0) + lane; b <= last; b += 32) {
-        const int rows = pa_rows(a, b), base = pa_kv(a, b) - pa_q(a, b);
-        const int t0 = max(0, it.tok0 - a.q_start[b]), t1 = min(rows, it.tok0 + it.ntok - a.q_start[b]);
+    int first = 0, last = a.n_req - 1, low = INT32_MAX;
+    if (a.n_req > 256) {  // two lanes search at once; fewer requests are looked at without a search (its loads follow one another)
+        const int edge = pa_request(a, lane & 1 ? tok0 + ntok - 1 : tok0);
+        first = __shfl_sync(0xffffffffu, edge, 0);
+        last = __shfl_sync(0xffffffffu, edge, 1);
+    }
+#pragma unroll 2
+    for (int b = first + lane; b <= last; b += 32) {
+        const int start = a.q_start[b], rows = pa_rows(a, b), base = pa_kv(a, b) - pa_q(a, b);
+        const int t0 = max(0, tok0 - start), t1 = min(rows, tok0 + ntok - start);
         if (t0 < t1 && base + t1 > 0 && !pa_inline(p, rows)) low = min(low, max(0, base + t0));
     }
     low = __reduce_min_sync(0xffffffffu, low);
-    return low == INT32_MAX ? P : min(P, max(0, P + low + 1 - a.window));
+    return low == INT32_MAX ? a.prefix_len : min(a.prefix_len, max(0, a.prefix_len + low + 1 - a.window));
 }
 
 // Item number i of the launch; false if it holds nothing (prefix rows of an inline request).  The TMA warp does this, ahead
@@ -247,7 +253,7 @@ __device__ __forceinline__ bool pa_item(const PaArgs& p, const int* ustart, int 
         it.pair = it.ntok > p.TPT;
         it.direct = false;
         it.npt = p.np;
-        it.klo_p = W > 0 ? pa_prefix_first(p, it, lane) : 0;
+        it.klo_p = W > 0 ? pa_prefix_first(p, it.tok0, it.ntok, lane) : 0;
         it.klo_o = it.khi_o = 0;
         it.v0 = max(c * p.ct_pre, it.klo_p / kPaKeys);
         it.n = max(0, min(p.np, (c + 1) * p.ct_pre) - it.v0);

@@ -43,3 +43,22 @@ def test_gone_pages_are_no_error(pg, kv, q, prefix, window, page):
         c["table"][b, :max(0, max(0, k - n) + 1 - window) // page] = -1
     check_attention(pg, c, dict(window=window))
     assert error_word() == 0
+
+
+@pytest.mark.parametrize("heads,hk", [(2, 2), (8, 1)])
+def test_many_requests(pg, heads, hk):
+    """More requests than the kernel looks at one by one: several row tiles, each with a least position of its own."""
+    import numpy as np
+    import torch
+    rng = np.random.default_rng(heads)
+    n, prefix, window = 600, 500, 300
+    kv = rng.integers(130, 180, n).tolist()
+    q = [int(x) for x in rng.integers(0, 3, n)]
+    c = make_case(kv, q, heads, hk, 64, 16, "float16", prefix=prefix, seed=heads)
+    p = torch.arange(first_seen(c, window))
+    at = (c["prefix_table"][p // 16].long(), p % 16)
+    c["k_pages"][at] = float("nan")
+    c["v_pages"][at] = float("inf")
+    c["prefix_table"][:len(p) // 16] = -1
+    check_attention(pg, c, dict(window=window))
+    assert error_word() == 0
