@@ -1218,7 +1218,8 @@ __global__ void __launch_bounds__(kRwThreads) k_pattn_rows(const __grid_constant
     const int chunks = pa_chunks(p, kv, false, &size);
     if (c >= chunks) return;
     const int q0 = max(a.q_start[b], 0), base = kv - q, nrow = n_tok * G;
-    const int hi = min(max(base + n_tok, 0), min(kv, (c + 1) * size * kPaKeys)), lo = W > 0 ? max(0, base + 1 - W) : 0;
+    // the last chunk's end would pass 32 bits in the longest contexts
+    const int hi = min(max(base + n_tok, 0), c + 1 < chunks ? (c + 1) * size * kPaKeys : kv), lo = W > 0 ? max(0, base + 1 - W) : 0;
     const int first = max(c * size * kPaKeys, lo & ~(kRwKeys - 1));
     const int n = first < hi ? (hi - first + kRwKeys - 1) / kRwKeys : 0;
     T* qsm = reinterpret_cast<T*>(rsm);
