@@ -83,8 +83,11 @@ struct PlanArgs {
     int* err;
 };
 
-// Sum of two that are not negative, at most INT32_MAX (so that sums of lengths out of range still ascend).
-__device__ __forceinline__ int add_sat(int x, int y) { return (int)min((unsigned)x + (unsigned)y, (unsigned)INT32_MAX); }
+// Sum of two that are not negative; of tokens at most INT32_MAX (so that sums of lengths out of range still ascend; those of
+// pages stay below it by the sizes that a plan takes).
+__device__ __forceinline__ int plan_add(bool tokens, int x, int y) {
+    return tokens ? (int)min((unsigned)x + (unsigned)y, (unsigned)INT32_MAX) : x + y;
+}
 
 // Last b in [0, n) with start[b] <= k (start ascends, start[0] = 0).
 __device__ __forceinline__ int owner(const int* start, int n, int k) {
@@ -107,13 +110,13 @@ __global__ void __launch_bounds__(kPlanThreads) k_pages_plan(const PlanArgs a) {
     const cg::cluster_group cluster = cg::this_cluster();
     const int gtid = (int)cluster.block_rank() * kPlanThreads + tid, gn = (int)cluster.num_blocks() * kPlanThreads;
     const int cap = a.table_ld * a.page_size;
-    const int free0 = *a.n_free, count0 = min(max(free0, 0), a.n_pages), room = a.n_pages - count0;
+    const int free0 = *a.n_free;
 
     // sums: each thread takes `per` consecutive requests
     const int per = (n + kPlanThreads - 1) / kPlanThreads;
     const int b0 = min(n, tid * per), b1 = min(n, b0 + per);
     int s[3] = {0, 0, 0};
-    bool bad = free0 != count0;
+    bool bad = false;
     for (int b = b0; b < b1; ++b) {
         int kv = a.kv_len[b], q = a.q_len[b];
         if (kv < 0 || kv > cap) bad = true, kv = min(max(kv, 0), cap);
@@ -126,7 +129,7 @@ __global__ void __launch_bounds__(kPlanThreads) k_pages_plan(const PlanArgs a) {
         back[b] = v[0], want[b] = v[1], toks[b] = v[2];
         base[b] = min(had, need);
 #pragma unroll
-        for (int i = 0; i < 3; ++i) s[i] = add_sat(s[i], v[i]);
+        for (int i = 0; i < 3; ++i) s[i] = plan_add(i == 2, s[i], v[i]);
     }
     int incl[3];
 #pragma unroll
@@ -135,7 +138,7 @@ __global__ void __launch_bounds__(kPlanThreads) k_pages_plan(const PlanArgs a) {
 #pragma unroll
         for (int o = 1; o < 32; o <<= 1) {
             const int u = __shfl_up_sync(0xffffffffu, incl[i], o);
-            if (lane >= o) incl[i] = add_sat(incl[i], u);
+            if (lane >= o) incl[i] = plan_add(i == 2, incl[i], u);
         }
         if (lane == 31) wsum[i][warp] = incl[i];
     }
@@ -147,24 +150,26 @@ __global__ void __launch_bounds__(kPlanThreads) k_pages_plan(const PlanArgs a) {
 #pragma unroll
         for (int w = 0; w < kPlanThreads / 32; ++w) {
             const int u = wsum[i][w];
-            before = w < warp ? add_sat(before, u) : before;
-            all = add_sat(all, u);
+            before = w < warp ? plan_add(i == 2, before, u) : before;
+            all = plan_add(i == 2, all, u);
         }
         tot[i] = all;
-        const int up = __shfl_up_sync(0xffffffffu, incl[i], 1);  // of the lanes in front
-        int run = lane ? add_sat(before, up) : before;
+        int in_front = incl[i] - s[i];
+        if (i == 2) in_front = __shfl_up_sync(0xffffffffu, incl[i], 1);
+        int run = plan_add(i == 2, before, i == 2 && lane == 0 ? 0 : in_front);
         int* arr = i == 0 ? back : i == 1 ? want : toks;
         for (int b = b0; b < b1; ++b) {
             const int v = arr[b];
             arr[b] = run;
-            run = add_sat(run, v);
+            run = plan_add(i == 2, run, v);
         }
         if (tid == 0) arr[n] = all;
     }
     __syncthreads();
     const int n_back = tot[0], n_want = tot[1], n_tok = tot[2];
+    const int count0 = min(max(free0, 0), a.n_pages), room = a.n_pages - count0;
     const int count = count0 + min(n_back, room), left = max(count - n_want, 0);
-    if (n_back > room) bad = true;  // the stack would hold more pages than there are
+    if (free0 != count0 || n_back > room) bad = true;  // also: the stack would hold more pages than there are
     if (n_back | n_want) {
         cluster.sync();  // every CTA has read the old state
         for (unsigned k0 = gtid; k0 < (unsigned)n_back; k0 += 4 * gn) {
