@@ -123,9 +123,9 @@ __global__ void __launch_bounds__(128) k_pattn_general(const sd_attn_args a, int
 // The running maximum that O refers to moves only when a row's maximum rises by more than 2^8 (exact: O and the sum
 // refer to the same value), so O is rarely rescaled.  Every wait is bounded in time (sd_common.cuh).
 //
-// What bounds it.  One causal prompt of 9472 tokens, 32 / 8 heads of 128, no bias: 637 us, 1154 TFLOP/s (0.70 of the
-// measured burst rate of a matrix product, 0.83 of the sustained one, which this length of run is nearer to).  256 rows x
-// 128 keys take the tensor cores 2480 clk with S in halves of 64 keys (N = 64, bound by shared memory; 2050 in one
+// What bounds it.  One causal prompt of 9472 tokens, 32 / 8 heads of 128, no bias: 636 us, 1154 TFLOP/s in short bursts (0.70
+// of the measured burst rate of a matrix product); back to back under the power limit 734 us, 0.72 of the sustained one.
+// 256 rows x 128 keys take the tensor cores 2480 clk with S in halves of 64 keys (N = 64, bound by shared memory; 2050 in one
 // piece) and the exponentials 2048 clk; each softmax warp needs about 1900 clk per half, of them 500 to 1000 waiting for
 // its share of the exponentials.  With caps and biases the extra arithmetic per score bounds it.
 //
@@ -1337,7 +1337,8 @@ __global__ void __launch_bounds__(kRwThreads) k_pattn_rows(const __grid_constant
         bool rise = false;
         if (a.softcap > 0.f) {
             // as in k_pattn, the same choice for each score whatever its neighbours are: the quotient's error is a part of
-            // the cap, so small scores take the polynomial, whose error is a part of the score
+            // the cap, so small scores take the polynomial, whose error is a part of the score (and which is no slower: decode
+            // of 64 ragged contexts 194.0 us, 195.4 with the quotient for all)
             float2 x[NT][2];
             bool big = false;
 #pragma unroll
@@ -1558,7 +1559,7 @@ bool tc_able(const sd_attn_args& a) {
 }
 
 // How the work of a call is cut: depends on what the host knows only (counts and bounds), so a request's split
-// does not depend on the other requests' lengths.
+// does not depend on the other requests' kv_len.
 void pa_plan(const sd_attn_args& a, int sms, PaArgs* p) {
     p->a = a;
     p->G = a.n_heads / a.pool.n_kv_heads;
@@ -1582,7 +1583,7 @@ void pa_plan(const sd_attn_args& a, int sms, PaArgs* p) {
     } else {
         // many rows: whole rounds over the SMs, in key tiles of about 2.2 us.  A cut costs an item about 3 tiles more, and
         // the join reads and the items write O of every row in 32 bits once per split (about 4 TB/s; without that term
-        // 8 prompts behind a prefix of 8192 were cut in two and took 477 us, uncut 439)
+        // 8 prompts behind a prefix of 8192 were cut in two and took 477 us, uncut 439, in short bursts)
         const double join = (double)a.n_tokens * a.n_heads * (a.pool.head_dim * 8 + 16) / 4e12 / 2.2e-6;
         double best = 1e300;
         for (int n = 1; n <= 32; ++n) {

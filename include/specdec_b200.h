@@ -202,8 +202,9 @@ SD_API int sd_kv_append_dev(const sd_kv_pool *pool, const void *k, const void *v
  * id is outside the pool are not seen (recorded, unless the page lies outside the windows of all rows of the call).  K and
  * V of positions that no row sees may hold anything; those that some row of the request (of the prefix: of the call)
  * sees must be finite.
- * q_start ascends, the ranges do not overlap and end within n_tokens.  max_q and max_kv bound q_len and kv_len on the
- * host (they size the launch; a tight max_kv gives the better split); a longer request is cut there (recorded).
+ * q_start ascends and the ranges do not overlap: q_start[b] + q_len[b] <= q_start[b + 1], of requests without new tokens
+ * too; the last ends within n_tokens.  max_q and max_kv bound q_len and kv_len on the host (they size the launch; a tight
+ * max_kv gives the better split); a longer request is cut there (recorded).
  * head_dim a multiple of 8 up to 256 (64 and 128 with 16-byte aligned rows run on the tensor cores), n_heads a multiple of
  * n_kv_heads (at most 128 per kv head), q and out of the pool's type and not overlapping; softcap 0 or 1e-6..1e30 (capped
  * scores are right to 2^-20 of their value; where scale / softcap is below 2^-126 the plain kernel takes the call). */
@@ -489,9 +490,9 @@ SD_API int sd_batch_forward(sd_batch *b, const int32_t *tokens, int T, const int
  * in pages (sd_pages, sd_attention_dev) instead of one ring per stream.  Every sd_batch_* call works on it, counting a
  * stream's positions from the end of the prefix (position 0 is the first token behind it); max_seq is their number.
  * A forward gives back the pages of positions behind its last token (a stream that has finished while others decode keeps
- * its own); a stream's n-gram history and repetition window
- * do not reach into the prefix.  Logits agree with those of a plain batch over prefix + tokens within the batched path's
- * tolerance (5e-3 relative): both attend with single fp16 Q and P. */
+ * its own); a stream's n-gram history and repetition window do not reach into the prefix.  Logits agree with those of a
+ * plain batch over prefix + tokens within the batched path's tolerance (5e-3 relative): both attend with single fp16 Q and
+ * P, and the head outputs pass through fp16 here before they are quantised. */
 SD_API int sd_batch_create_shared(sd_ctx *ctx, const int32_t *prefix, int n_prefix, int n_streams, int max_seq,
                                   int max_width, sd_batch **out);
 /* K/V of positions [0, n) of every stream from tokens [n_streams][n] (chunks of max_width tokens). */
