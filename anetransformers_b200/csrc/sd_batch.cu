@@ -1469,7 +1469,7 @@ int sd_batch_decode(sd_batch* b, const sd_gen_params* gp, const int32_t* history
     t.hist_cap = cap;
     t.hlen = n_hist;
     t.rng_counter = 1ull << 20;
-    k_binit_gen<<<b->B, 256, 0, b->st>>>(b->gs, b->B, t, b->g_out, b->g_hist, cap, b->tok, n_hist, n_hist, cur, gp->seed);
+    k_binit_gen<<<b->B, 256, 0, b->st>>>(b->gs, b->B, t, b->g_out, b->g_hist, b->g_cap, b->tok, n_hist, n_hist, cur, gp->seed);
     CK(cudaGetLastError(), "state");
     // the first token counts as generated but is not in the output (sd_decode semantics)
     CK(launch_bgen_first_fixup(b->gs, b->B, p.gen_limit, p.ignore_eos, p.eos_id, b->st), "state");
@@ -1510,7 +1510,7 @@ int sd_batch_generate(sd_batch* b, const sd_gen_params* gp, const int32_t* promp
     t.out_cap = cap;
     t.hist_cap = cap;
     t.hlen = n_prompt;
-    k_binit_gen<<<b->B, 256, 0, b->st>>>(b->gs, b->B, t, b->g_out, b->g_hist, cap, b->tok, n_prompt, n_prompt, nullptr,
+    k_binit_gen<<<b->B, 256, 0, b->st>>>(b->gs, b->B, t, b->g_out, b->g_hist, b->g_cap, b->tok, n_prompt, n_prompt, nullptr,
                                          gp->seed);
     CK(cudaGetLastError(), "state");
     CK(launch_bgen_commit(b->gs, b->ctrl, b->B, b->logits, b->probs, b->argmax, p1, b->m.vocab, Tl, Tl - 1, b->st), "first token");
